@@ -45,6 +45,9 @@ OPS = {
     "diopiRMSNorm": [c_void_p, c_void_p, c_void_p, diopiSize_t, c_void_p, c_void_p, c_double],
     "diopiRotaryEmbeddingCopyKV": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_bool],
     "diopiMatmulAllReduce": [c_void_p, c_void_p, c_void_p, c_void_p, c_char_p, c_char_p, c_int64, c_int64],
+    "diopiBuildBlockTable": [c_void_p] * 10 + [c_int64],
+    "diopiQuantizedCopyKV": [c_void_p] * 9,
+    "diopiQuantizedPagedAttention": [c_void_p] * 8 + [c_double],
     "diopiB200ContextRelease": [],
     "diopiRMSNormBackward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, diopiSize_t, c_double],
 }

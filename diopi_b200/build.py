@@ -45,6 +45,9 @@ IMPL_SOURCES = [
     "kernels/context_attention.cu",
     "kernels/context_attention_sm100.cu",
     "kernels/matmul_allreduce.cu",
+    "kernels/block_table.cu",
+    "kernels/quantized_copy_kv.cu",
+    "kernels/quantized_attention.cu",
 ]
 RT_SOURCES = ["rt/testrt.cpp"]
 

@@ -275,9 +275,10 @@ void restore_async_status(int v) {
 void fail_with_async_status(int v) {
     const char* what = "unknown";
     switch (v) {
-        case 1: what = "a pool slot index read from b_loc or dest_loc was outside the pool; that row was skipped"; break;
+        case 1: what = "a pool slot index read from b_loc or dest_loc, or a block of a block table, was outside the pool; that row was skipped"; break;
         case 2: what = "a token id passed to diopiApplyPenalty was outside the vocabulary; that entry was skipped"; break;
         case 3: what = "a kernel gave up a bounded wait (its own memory pipeline, or the rows of a tensor-parallel peer)"; break;
+        case 4: what = "diopiBuildBlockTable ran out of free blocks, or a request or its slots outgrew the tables; those entries were marked as missing"; break;
         default: break;
     }
     fail(diopiErrorOccurred, "an earlier kernel of this library reported status %d: %s (this call itself was launched)", v, what);

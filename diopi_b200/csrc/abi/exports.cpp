@@ -979,3 +979,260 @@ B200_EXPORT diopiError_t diopiPagedAttention(diopiContextHandle_t ctx, diopiTens
         B200_CUDA(cudaGetLastError());
     });
 }
+
+// ---------------------------------------------------------------------------------------------
+// A block-paged K/V cache held in 8 bits: tables from lengths, the store, and the attention over it.
+// ---------------------------------------------------------------------------------------------
+namespace {
+
+// First and last byte that a view can touch.
+void byte_range(const TensorView& t, uintptr_t& lo, uintptr_t& hi) {
+    const int64_t e = t.elem_size();
+    lo = hi = reinterpret_cast<uintptr_t>(t.data);
+    if (t.numel == 0) return;
+    for (int i = 0; i < t.ndim; ++i) {
+        const int64_t reach = (t.shape[i] - 1) * t.stride[i] * e;
+        if (reach >= 0)
+            hi += static_cast<uintptr_t>(reach);
+        else
+            lo -= static_cast<uintptr_t>(-reach);
+    }
+    hi += static_cast<uintptr_t>(e);
+}
+
+bool overlap(const TensorView& a, const TensorView& b) {
+    if (!a.defined || !b.defined || a.numel == 0 || b.numel == 0) return false;
+    uintptr_t al, ah, bl, bh;
+    byte_range(a, al, ah);
+    byte_range(b, bl, bh);
+    return al < bh && bl < ah;
+}
+
+// Elements of a tensor that a kernel writes must not share memory: an expanded dim would make rows of it one.
+void written(const TensorView& t, const char* name) {
+    for (int i = 0; i < t.ndim; ++i)
+        B200_REQUIRE(t.shape[i] <= 1 || t.stride[i] != 0, "'%s' is written and must not have an expanded dim", name);
+}
+
+// The two caches and their scales: dtype, shapes, strides.
+struct CacheViews {
+    TensorView cache[2], scale[2];
+    bool e4m3;
+    int64_t blocks;
+    int block_size, H, D;
+};
+
+CacheViews cache_views(diopiConstTensorHandle_t kc, diopiConstTensorHandle_t vc, diopiConstTensorHandle_t ks, diopiConstTensorHandle_t vs) {
+    CacheViews c;
+    const char* cn[2] = {"k_cache", "v_cache"};
+    const char* sn[2] = {"k_scale", "v_scale"};
+    c.cache[0] = view_of(kc, cn[0]);
+    c.cache[1] = view_of(vc, cn[1]);
+    c.scale[0] = view_of(ks, sn[0]);
+    c.scale[1] = view_of(vs, sn[1]);
+    for (int m = 0; m < 2; ++m) {
+        const TensorView& t = c.cache[m];
+        if (t.dtype != diopi_dtype_int8 && t.dtype != diopi_dtype_uint8)
+            fail(diopiDtypeNotSupported, "'%s' has dtype %s; expected int8, or uint8 holding e4m3 bits", cn[m], dtype_name(t.dtype));
+        B200_REQUIRE(t.ndim == 4, "'%s' must be [blocks, block_size, kv_heads, head_dim], got %d dims", cn[m], t.ndim);
+        if (c.scale[m].dtype != diopi_dtype_float32) fail(diopiDtypeNotSupported, "'%s' has dtype %s; expected float32", sn[m], dtype_name(c.scale[m].dtype));
+        B200_REQUIRE(c.scale[m].ndim == 2 && c.scale[m].shape[0] == t.shape[0] && c.scale[m].shape[1] == t.shape[2], "'%s' must be [%ld, %ld]", sn[m],
+                     (long)t.shape[0], (long)t.shape[2]);
+    }
+    same_dtype(c.cache[1], cn[1], c.cache[0], cn[0]);
+    for (int i = 0; i < 4; ++i) B200_REQUIRE(c.cache[0].shape[i] == c.cache[1].shape[i], "'k_cache' and 'v_cache' differ in dim %d", i);
+    const int64_t* s = c.cache[0].shape;
+    B200_REQUIRE(s[1] > 0 && s[1] < (1ll << 30) && s[2] > 0 && s[2] <= 65535 && s[3] > 0, "'k_cache' is [%ld, %ld, %ld, %ld]: block_size, kv_heads and head_dim must be positive",
+                 (long)s[0], (long)s[1], (long)s[2], (long)s[3]);
+    B200_REQUIRE(s[3] <= 512, "head_dim %ld is beyond the supported maximum of 512", (long)s[3]);
+    c.e4m3 = c.cache[0].dtype == diopi_dtype_uint8;
+    c.blocks = s[0];
+    c.block_size = static_cast<int>(s[1]);
+    c.H = static_cast<int>(s[2]);
+    c.D = static_cast<int>(s[3]);
+    return c;
+}
+
+int table_cols(const TensorView& t, int64_t block_size) {
+    B200_REQUIRE(t.shape[1] * block_size < (1ll << 31), "'block_table' covers %ld tokens of a request; at most 2^31 - 1 are supported",
+                 (long)(t.shape[1] * block_size));
+    return static_cast<int>(t.shape[1]);
+}
+
+}  // namespace
+
+B200_EXPORT diopiError_t diopiBuildBlockTable(diopiContextHandle_t ctx, diopiTensorHandle_t block_table, diopiTensorHandle_t slot_map,
+                                              diopiTensorHandle_t new_start, diopiTensorHandle_t seq_lens, diopiTensorHandle_t token_table,
+                                              diopiTensorHandle_t free_next, diopiConstTensorHandle_t cached_lens, diopiConstTensorHandle_t new_lens,
+                                              diopiConstTensorHandle_t free_blocks, diopiConstTensorHandle_t free_start, int64_t block_size) {
+    return guard("diopiBuildBlockTable", [&] {
+        flush_pending(ctx);
+        const char* names[] = {"block_table", "slot_map", "new_start", "seq_lens", "free_next", "token_table", "cached_lens", "new_lens", "free_blocks", "free_start"};
+        TensorView v[] = {view_of(block_table, names[0]), view_of(slot_map, names[1]), view_of(new_start, names[2]), view_of(seq_lens, names[3]),
+                          view_of(free_next, names[4]), view_of(token_table, names[5], /*optional=*/true), view_of(cached_lens, names[6]),
+                          view_of(new_lens, names[7]), view_of(free_blocks, names[8]), view_of(free_start, names[9])};
+        constexpr int kOutputs = 6, kAll = 10;
+        k::BlockTableArgs a{};
+        a.table = index_arg(v[0], names[0], 2);
+        a.slot_map = index_arg(v[1], names[1], 1);
+        a.new_start = index_arg(v[2], names[2], 1);
+        a.seq_lens = index_arg(v[3], names[3], 1);
+        a.free_next = index_arg(v[4], names[4], 1);
+        if (v[5].defined) a.wide = index_arg(v[5], names[5], 2);
+        a.cached = index_arg(v[6], names[6], 1);
+        a.fresh = index_arg(v[7], names[7], 1);
+        a.free_blocks = index_arg(v[8], names[8], 1);
+        a.free_start = index_arg(v[9], names[9], 1);
+        B200_REQUIRE(block_size > 0 && block_size < (1ll << 30), "block_size must be positive (got %ld)", (long)block_size);
+        const int64_t B = v[0].shape[0];
+        B200_REQUIRE(B < (1ll << 30), "the batch has %ld requests; at most 2^30 - 1 are supported", (long)B);
+        B200_REQUIRE(v[3].shape[0] == B && v[6].shape[0] == B && v[7].shape[0] == B, "'seq_lens', 'cached_lens' and 'new_lens' must have batch = %ld entries", (long)B);
+        B200_REQUIRE(v[2].shape[0] == B + 1, "'new_start' must have batch + 1 = %ld entries, got %ld", (long)(B + 1), (long)v[2].shape[0]);
+        B200_REQUIRE(v[4].shape[0] == 1 && v[9].shape[0] == 1, "'free_next' and 'free_start' must have one entry");
+        if (v[5].defined) B200_REQUIRE(v[5].shape[0] == B, "'token_table' has %ld rows for a batch of %ld", (long)v[5].shape[0], (long)B);
+        for (int i = 0; i < kOutputs; ++i) {
+            if (!v[i].defined) continue;
+            written(v[i], names[i]);
+            for (int j = i + 1; j < kAll; ++j) B200_REQUIRE(!overlap(v[i], v[j]), "'%s' and '%s' must not share memory", names[i], names[j]);
+        }
+        a.B = static_cast<int>(B);
+        a.cols = table_cols(v[0], block_size);
+        a.block_size = static_cast<int>(block_size);
+        a.T = v[1].shape[0];
+        a.wide_cols = v[5].defined ? v[5].shape[1] : 0;
+        if (a.wide_cols == 0) a.wide = k::IndexArg{};
+        a.n_free = v[8].shape[0];
+        cudaStream_t st = stream_of(ctx);
+        const DeviceInfo& di = device_info();
+        a.status = async_status_device_ptr();
+        k::launch_block_table(a, di.sm_count, st);
+        B200_CUDA(cudaGetLastError());
+    });
+}
+
+B200_EXPORT diopiError_t diopiQuantizedCopyKV(diopiContextHandle_t ctx, diopiTensorHandle_t k_cache, diopiTensorHandle_t v_cache,
+                                              diopiTensorHandle_t k_scale, diopiTensorHandle_t v_scale, diopiConstTensorHandle_t kh,
+                                              diopiConstTensorHandle_t vh, diopiConstTensorHandle_t block_table, diopiConstTensorHandle_t cached_lens,
+                                              diopiConstTensorHandle_t new_start) {
+    return guard("diopiQuantizedCopyKV", [&] {
+        flush_pending(ctx);
+        const CacheViews c = cache_views(k_cache, v_cache, k_scale, v_scale);
+        const TensorView src[2] = {view_of(kh, "k"), view_of(vh, "v")};
+        const TensorView bt = view_of(block_table, "block_table"), cl = view_of(cached_lens, "cached_lens"), ns = view_of(new_start, "new_start");
+        k::QuantCopyArgs a{};
+        a.dt = float_dt(src[0], "k", false);
+        same_dtype(src[1], "v", src[0], "k");
+        for (int m = 0; m < 2; ++m) {
+            const char* name = m ? "v" : "k";
+            B200_REQUIRE(src[m].ndim == 3 && src[m].shape[0] == src[0].shape[0] && src[m].shape[1] == c.H && src[m].shape[2] == c.D, "'%s' must be [tokens, %d, %d]", name,
+                         c.H, c.D);
+            written(c.cache[m], m ? "v_cache" : "k_cache");
+            written(c.scale[m], m ? "v_scale" : "k_scale");
+            a.src[m] = src[m].data;
+            a.src_s0[m] = src[m].stride[0];
+            a.src_s1[m] = src[m].stride[1];
+            a.src_s2[m] = src[m].stride[2];
+            a.cache[m] = c.cache[m].data;
+            a.c_s0[m] = c.cache[m].stride[0];
+            a.c_s1[m] = c.cache[m].stride[1];
+            a.c_s2[m] = c.cache[m].stride[2];
+            a.c_s3[m] = c.cache[m].stride[3];
+            a.scale[m] = static_cast<float*>(c.scale[m].data);
+            a.s_s0[m] = c.scale[m].stride[0];
+            a.s_s1[m] = c.scale[m].stride[1];
+        }
+        // K and V may be interleaved views of one allocation, but not the same elements.
+        B200_REQUIRE(c.cache[0].numel == 0 || c.cache[0].data != c.cache[1].data, "'k_cache' and 'v_cache' are the same memory");
+        B200_REQUIRE(c.scale[0].numel == 0 || c.scale[0].data != c.scale[1].data, "'k_scale' and 'v_scale' are the same memory");
+        a.table = index_arg(bt, "block_table", 2);
+        a.cached = index_arg(cl, "cached_lens", 1);
+        a.new_start = index_arg(ns, "new_start", 1);
+        const int64_t B = bt.shape[0];
+        B200_REQUIRE(B < (1ll << 28), "the batch has %ld requests; at most 2^28 - 1 are supported", (long)B);
+        B200_REQUIRE(cl.shape[0] == B, "'cached_lens' must have batch = %ld entries, got %ld", (long)B, (long)cl.shape[0]);
+        B200_REQUIRE(ns.shape[0] == B + 1, "'new_start' must have batch + 1 = %ld entries, got %ld", (long)(B + 1), (long)ns.shape[0]);
+        B200_REQUIRE(src[0].shape[0] < (1ll << 30), "'k' has %ld rows; at most 2^30 - 1 are supported", (long)src[0].shape[0]);
+        a.e4m3 = c.e4m3;
+        a.B = static_cast<int>(B);
+        a.cols = table_cols(bt, c.block_size);
+        a.block_size = c.block_size;
+        a.H = c.H;
+        a.D = c.D;
+        a.T = src[0].shape[0];
+        a.blocks = c.blocks;
+        if (B == 0 || a.T == 0) return;
+        cudaStream_t st = stream_of(ctx);
+        device_info();
+        a.status = async_status_device_ptr();
+        k::launch_quantized_copy_kv(a, st);
+        B200_CUDA(cudaGetLastError());
+    });
+}
+
+B200_EXPORT diopiError_t diopiQuantizedPagedAttention(diopiContextHandle_t ctx, diopiTensorHandle_t out, diopiConstTensorHandle_t q,
+                                                      diopiConstTensorHandle_t k_cache, diopiConstTensorHandle_t v_cache,
+                                                      diopiConstTensorHandle_t k_scale, diopiConstTensorHandle_t v_scale,
+                                                      diopiConstTensorHandle_t block_table, diopiConstTensorHandle_t seq_lens, double softmax_scale) {
+    return guard("diopiQuantizedPagedAttention", [&] {
+        flush_pending(ctx);
+        const TensorView o = view_of(out, "out"), qv = view_of(q, "q"), bt = view_of(block_table, "block_table"), sl = view_of(seq_lens, "seq_lens");
+        const CacheViews c = cache_views(k_cache, v_cache, k_scale, v_scale);
+        k::QuantAttnArgs a{};
+        a.dt = float_dt(qv, "q", false);
+        same_dtype(o, "out", qv, "q");
+        const int nd = qv.ndim;
+        B200_REQUIRE((nd == 3 || nd == 4) && o.ndim == nd, "'q' and 'out' must be [batch, heads, head_dim] or [batch, tokens, heads, head_dim]");
+        for (int i = 0; i < nd; ++i) B200_REQUIRE(o.shape[i] == qv.shape[i], "'q' and 'out' differ in dim %d", i);
+        const int64_t B = qv.shape[0], n = nd == 4 ? qv.shape[1] : 1, Hq = qv.size(-2), D = qv.size(-1);
+        B200_REQUIRE(D == c.D, "'q' has head_dim %ld, the cache %d", (long)D, c.D);
+        B200_REQUIRE(Hq > 0 && Hq % c.H == 0, "the %ld heads of 'q' must be a positive multiple of the cache's %d", (long)Hq, c.H);
+        B200_REQUIRE(n * Hq <= 65535, "tokens * heads of 'q' is %ld; at most 65535 are supported", (long)(n * Hq));
+        B200_REQUIRE(D == 1 || (qv.str(-1) == 1 && o.str(-1) == 1), "the last dim of 'q' and 'out' must be dense");
+        written(o, "out");
+        B200_REQUIRE(!overlap(o, qv) || (o.data == qv.data && same_tensor(o, qv)), "'out' may be 'q' itself, but not overlap it otherwise");
+        B200_REQUIRE(std::isfinite(softmax_scale) && softmax_scale > 0 && softmax_scale < 1e30, "softmax_scale must be positive and finite (got %g)", softmax_scale);
+        a.table = index_arg(bt, "block_table", 2);
+        a.lens = index_arg(sl, "seq_lens", 1);
+        B200_REQUIRE(bt.shape[0] == B && sl.shape[0] == B, "'block_table' and 'seq_lens' must have batch = %ld rows", (long)B);
+        B200_REQUIRE(B < (1ll << 28), "the batch has %ld requests; at most 2^28 - 1 are supported", (long)B);
+        a.q = qv.data;
+        a.q_s0 = qv.stride[0];
+        a.q_s1 = nd == 4 ? qv.stride[1] : 0;
+        a.q_s2 = qv.str(-2);
+        a.out = o.data;
+        a.o_s0 = o.stride[0];
+        a.o_s1 = nd == 4 ? o.stride[1] : 0;
+        a.o_s2 = o.str(-2);
+        for (int m = 0; m < 2; ++m) {
+            a.cache[m] = c.cache[m].data;
+            a.c_s0[m] = c.cache[m].stride[0];
+            a.c_s1[m] = c.cache[m].stride[1];
+            a.c_s2[m] = c.cache[m].stride[2];
+            a.c_s3[m] = c.cache[m].stride[3];
+            a.scale[m] = static_cast<const float*>(c.scale[m].data);
+            a.s_s0[m] = c.scale[m].stride[0];
+            a.s_s1[m] = c.scale[m].stride[1];
+        }
+        a.e4m3 = c.e4m3;
+        a.B = static_cast<int>(B);
+        a.n = static_cast<int>(n);
+        a.Hq = static_cast<int>(Hq);
+        a.Hkv = c.H;
+        a.D = c.D;
+        a.block_size = c.block_size;
+        a.cols = table_cols(bt, c.block_size);
+        a.blocks = c.blocks;
+        a.softmax_scale = static_cast<float>(softmax_scale);
+        a.force_plain = options().decode_plain;
+        if (qv.numel == 0) return;
+        cudaStream_t st = stream_of(ctx);
+        const DeviceInfo& di = device_info();
+        a.status = async_status_device_ptr();
+        const int64_t ws_bytes = k::quantized_attention_workspace_bytes(a, di.sm_count, di.max_smem_optin);
+        void* ws = ws_bytes > 0 ? workspace(ctx, ws_bytes) : nullptr;
+        const char* kernel = k::launch_quantized_attention(a, ws, di.sm_count, di.max_smem_optin, st);
+        logf("quantized paged attention B=%d tokens=%d heads=%d/%d D=%d block=%d scratch=%ld bytes (%s kernel)", a.B, a.n, a.Hq, a.Hkv, a.D, a.block_size,
+             (long)ws_bytes, kernel);
+        B200_CUDA(cudaGetLastError());
+    });
+}

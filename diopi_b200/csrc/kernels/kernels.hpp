@@ -65,6 +65,60 @@ void launch_decode(const DecodeArgs& a, void* ws, int sm_count, int max_smem, cu
 int64_t decode_static_scratch_capacity();
 cudaError_t launch_decode_static_scratch(const DecodeArgs& a, int sm_count, int max_smem, cudaStream_t st, int64_t* needed);
 
+// ---- block tables and slot maps of a paged cache, from request lengths --------
+constexpr int32_t kNoSlot = INT32_MIN;   // outside every pool, also for the ops that count negative slots from the end
+struct BlockTableArgs {
+    IndexArg table;            // [B, cols]: entries of blocks held are read, entries of blocks taken are written
+    IndexArg slot_map;         // [T], written
+    IndexArg new_start;        // [B + 1], written
+    IndexArg seq_lens;         // [B], written
+    IndexArg wide;             // [B, wide_cols] right-aligned, written; ptr null: not wanted
+    IndexArg free_next;        // [1], written
+    IndexArg cached, fresh;    // [B] tokens held already, tokens that come in
+    IndexArg free_blocks;      // [n_free]
+    IndexArg free_start;       // [1]
+    int B, cols, block_size;
+    int64_t T, wide_cols, n_free;
+    int* status;
+};
+void launch_block_table(const BlockTableArgs& a, int sm_count, cudaStream_t st);
+
+// ---- paged cache in 8 bits, one fp32 scale for each (block, K/V head) ---------
+// A code c of a block with scale s stands for c * s: int8, or the bits of an e4m3 value.
+struct QuantCopyArgs {
+    Dt dt;                                               // of the new rows
+    const void* src[2]; int64_t src_s0[2], src_s1[2], src_s2[2];   // K, V: [T, H, D], strides in elements
+    void* cache[2]; int64_t c_s0[2], c_s1[2], c_s2[2], c_s3[2];    // [blocks, block_size, H, D], strides in bytes
+    float* scale[2]; int64_t s_s0[2], s_s1[2];           // [blocks, H]
+    bool e4m3;
+    IndexArg table;                                      // [B, cols]
+    IndexArg cached;                                     // [B]
+    IndexArg new_start;                                  // [B + 1]
+    int B, cols, block_size, H, D;
+    int64_t T, blocks;
+    int* status;
+};
+void launch_quantized_copy_kv(const QuantCopyArgs& a, cudaStream_t st);
+
+struct QuantAttnArgs {
+    Dt dt;                                               // of q and out
+    const void* q; int64_t q_s0, q_s1, q_s2;             // [B, n, Hq, D], last dim dense
+    void* out; int64_t o_s0, o_s1, o_s2;
+    const void* cache[2]; int64_t c_s0[2], c_s1[2], c_s2[2], c_s3[2];   // K, V codes, strides in bytes
+    const float* scale[2]; int64_t s_s0[2], s_s1[2];
+    bool e4m3;
+    IndexArg table, lens;
+    int B, n, Hq, Hkv, D, block_size, cols;
+    int64_t blocks;
+    float softmax_scale;
+    int force_plain;
+    int* status;
+};
+// Bytes of scratch for these arguments, 0 where they take the plain kernel (which needs none).
+int64_t quantized_attention_workspace_bytes(const QuantAttnArgs& a, int sm_count, int max_smem);
+// Returns the name of the kernel that took the call ("split", "plain").
+const char* launch_quantized_attention(const QuantAttnArgs& a, void* ws, int sm_count, int max_smem, cudaStream_t st);
+
 // ---- RMSNorm ----------------------------------------------------------------
 struct RmsNormArgs {
     Dt dt;

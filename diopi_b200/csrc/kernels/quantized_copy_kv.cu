@@ -1,0 +1,405 @@
+// New K and V rows into a paged cache of 8-bit codes with one scale for each (block, head) (diopiQuantizedCopyKV).
+//
+// A block whose first position is written by the call begins anew: with amax the largest magnitude of the call's rows in it
+//     int8:  s = max(fp32(amax / 127), 2^-126)         e4m3:  s = 2^k, the smallest k >= -126 with amax <= 448 * 2^k
+// (s = 0 when amax = 0). A block that an earlier call began keeps its tokens: its scale becomes s' = s * 2^k with the
+// smallest k >= 0 that covers the new rows, and the codes in front of them become rne(code * 2^-k). Growth by powers of two
+// keeps that exact where the format can hold the result, so that a block filled token by token does not drift. A new code is
+// the correctly rounded quotient x / s, ties to even; all of it is a function of the values alone, so that any order of
+// the work gives the same bits. NaN and infinities do not count into amax: they saturate (int8 NaN: 0, e4m3 NaN: NaN).
+//
+// Bytes: T * H * D * (e + 1) for each of K and V. One pass: the rows of a block stay in registers between the maximum and
+// the codes. A unit is one (request, block, head) of one matrix; 16 rows of it belong to a warp, with 16 elements of a row to
+// a lane (one 16-byte store of codes), and ceil(block_size / 16) warps (up to 8) share a unit through shared memory. Blocks
+// of more than 128 rows are read twice (the second time from L1/L2).
+#include <cuda_fp8.h>
+
+#include <type_traits>
+
+#include "dev_util.cuh"
+
+namespace b200 {
+namespace k {
+namespace {
+
+constexpr int kCopyThreads = 256;
+constexpr int kCopyWarps = kCopyThreads / 32;
+constexpr int kWarpRows = 16;
+constexpr float kFltMin = 1.17549435e-38f;   // 2^-126
+
+// The scale of a block that begins anew.
+__device__ __forceinline__ float fresh_scale(float amax, bool e4m3) {
+    if (!(amax > 0.f)) return 0.f;
+    if (!e4m3) return fmaxf(__fdiv_rn(amax, 127.f), kFltMin);
+    const uint32_t u = __float_as_uint(amax);
+    const int e = static_cast<int>(u >> 23);                       // biased; 0 for subnormals
+    int k = e - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);         // 448 = 1.75 * 2^8
+    k = e == 0 ? 1 : max(k, 1);                                    // 2^-126 at least
+    return __uint_as_float(static_cast<uint32_t>(k) << 23);
+}
+
+// Smallest k >= 0 with old * 2^k >= need. The quotient of two fp32 values is further from any power of two than the
+// rounding of a double, unless it is one.
+__device__ __forceinline__ int growth_steps(float old, float need) {
+    if (!(need > old)) return 0;
+    const double r = static_cast<double>(need) / static_cast<double>(old);
+    const int hi = __double2hiint(r), lo = __double2loint(r);
+    return ((hi >> 20) & 0x7ff) - 1023 + (((hi & 0xfffff) | lo) != 0 ? 1 : 0);
+}
+
+__device__ __forceinline__ float pow2f(int k) { return k < -149 ? 0.f : exp2f(static_cast<float>(k)); }
+
+// One value, any input: the definition itself in double (a quotient of two fp32 values is never close enough to a tie of
+// an 8-bit format, without being one, for the double rounding to matter).
+__device__ __noinline__ uint32_t encode_slow(float x, float s, bool e4m3) {
+    if (e4m3) {
+        if (isnan(x)) return 0x7fu;
+        if (s == 0.f) return 0u;
+        const float y = static_cast<float>(static_cast<double>(x) / static_cast<double>(s));   // s is a power of two
+        return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+    }
+    if (isnan(x) || s == 0.f) return 0u;
+    double y = rint(static_cast<double>(x) / static_cast<double>(s));
+    y = y > 127. ? 127. : (y < -127. ? -127. : y);
+    return static_cast<uint32_t>(static_cast<int>(y)) & 0xffu;
+}
+
+__device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Four codes. `inv` = 1 / s (exact for the powers of two of e4m3). int8: adding 1.5 * 2^23 rounds x * inv to an integer,
+// which sits in the low byte; x * inv carries the error of inv, so where the remainder x - q * s (exact in one fma: |q| <=
+// 127) is half a step or more the nearest code may be another one and `off` asks for the slow path.
+__device__ __forceinline__ uint32_t encode4(const float* x, float s, float inv, bool e4m3, float& off) {
+    if (e4m3) return e4m3_pair(x[0] * inv, x[1] * inv) | (e4m3_pair(x[2] * inv, x[3] * inv) << 16);
+    constexpr float kMagic = 12582912.f;
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float t = fmaf(x[i], inv, kMagic);
+        off = fmaxf(off, fabsf(fmaf(-(t - kMagic), s, x[i])));
+        b[i] = __float_as_uint(t);
+    }
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+
+// A code in a scale that has grown by 2^k; f = 2^-k.
+__device__ __forceinline__ uint32_t shrink_code(uint32_t c, float f, bool e4m3) {
+    if (e4m3) {
+        __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(c), __NV_E4M3);
+        return __nv_cvt_float_to_fp8(__half2float(__half(h)) * f, __NV_SATFINITE, __NV_E4M3);
+    }
+    return static_cast<uint32_t>(static_cast<int>(rintf(static_cast<float>(static_cast<int8_t>(c)) * f))) & 0xffu;
+}
+
+struct CopyUnit {
+    int64_t row0;        // first row of the call in this block
+    int64_t block;       // block id, -1: nothing to do
+    int p0, p1;          // positions written
+};
+
+// Finds unit u of the batch: the requests' touched blocks, one after the other. All threads of the CTA take part.
+__device__ __forceinline__ CopyUnit find_unit(const QuantCopyArgs& a, int u) {
+    __shared__ int warp_sum[kCopyWarps];
+    __shared__ int s_req, s_j;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t cap = static_cast<int64_t>(a.cols) * a.block_size;
+    if (tid == 0) s_req = -1;
+    int carry = 0;
+    CopyUnit un{0, -1, 0, 0};
+    for (int base = 0; base < a.B; base += kCopyThreads) {
+        const int r = base + tid;
+        int cnt = 0;
+        if (r < a.B) {
+            const int64_t c = load_index(a.cached, r);
+            const int64_t n = imin64(load_index(a.new_start, r + 1), a.T) - load_index(a.new_start, r);
+            if (u == 0 && n > 0 && (c < 0 || n > cap - c)) report_status(a.status, 1);   // the tokens that the table has no column for
+            if (n > 0 && c >= 0 && c < cap) cnt = static_cast<int>((c % a.block_size + imin64(n, cap - c) + a.block_size - 1) / a.block_size);
+        }
+        int v = cnt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int w = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += w;
+        }
+        if (lane == 31) warp_sum[warp] = v;
+        __syncthreads();
+        int total = 0, below = 0;
+#pragma unroll
+        for (int w = 0; w < kCopyWarps; ++w) {
+            below += w < warp ? warp_sum[w] : 0;
+            total += warp_sum[w];
+        }
+        const int first = carry + below + v - cnt;
+        if (u >= first && u < first + cnt) {
+            s_req = r;
+            s_j = u - first;
+        }
+        carry += total;
+        __syncthreads();
+        if (u > 0 && u < carry) break;
+    }
+    __syncthreads();
+    const int req = s_req;
+    if (req < 0) return un;
+    const int j = s_j;
+    const int64_t c = load_index(a.cached, req), t0 = load_index(a.new_start, req);
+    const int64_t n = imin64(imin64(load_index(a.new_start, req + 1), a.T) - t0, cap - c);
+    const int64_t b = c / a.block_size + j, lo = imax64(c, b * a.block_size), hi = imin64(c + n, (b + 1) * a.block_size);
+    const int64_t id = load_index(a.table, req, b);
+    if (id < 0 || id >= a.blocks || t0 < 0) {
+        if (tid == 0) report_status(a.status, 1);
+        return un;
+    }
+    un.row0 = t0 + (lo - c);
+    un.block = id;
+    un.p0 = static_cast<int>(lo - b * a.block_size);
+    un.p1 = static_cast<int>(hi - b * a.block_size);
+    return un;
+}
+
+// The 16 elements [16 * cl, 16 * cl + 16) of a row in fp32.
+template <typename T>
+struct Row16 {
+    static constexpr int N = 16 / Vec16<T>::N;   // 16-byte vectors
+    uint4 v[N];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void unpack(float (&f)[16]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float g[Vec16<T>::N];
+            unpack16<T>(v[i], g);
+#pragma unroll
+            for (int j = 0; j < Vec16<T>::N; ++j) f[i * Vec16<T>::N + j] = g[j];
+        }
+    }
+};
+
+// Lanes of a row LPR (power of two, 16 elements each; lanes beyond D / 16 idle), W warps of 16 rows to a unit.
+template <typename T, int LPR, int W, bool REREAD>
+__global__ void __launch_bounds__(kCopyThreads) quantized_copy_kernel(const QuantCopyArgs a) {
+    constexpr int RPP = 32 / LPR;              // rows of a warp's pass
+    constexpr int PASSES = kWarpRows / RPP;
+    constexpr int UPC = kCopyWarps / W;        // heads of a CTA
+    __shared__ float s_amax[kCopyWarps];
+    __shared__ int s_odd[kCopyWarps];
+    const int m = blockIdx.z;                  // 0: K, 1: V
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const CopyUnit un = find_unit(a, blockIdx.x);
+    if (un.block < 0) return;                  // the same for the whole CTA
+    const int h = blockIdx.y * UPC + warp / W, wu = warp % W;
+    const bool here = h < a.H;
+    const int rl = lane / LPR, cl = lane % LPR;
+    const bool col = here && cl * 16 < a.D;
+    const T* src = static_cast<const T*>(a.src[m]) + static_cast<int64_t>(h) * a.src_s1[m] + cl * 16;
+    uint8_t* dst = static_cast<uint8_t*>(a.cache[m]) + un.block * a.c_s0[m] + static_cast<int64_t>(h) * a.c_s2[m] + cl * 16;
+    float* scale = a.scale[m] + un.block * a.s_s0[m] + static_cast<int64_t>(h) * a.s_s1[m];
+
+    // Row of pass i of chunk q in the block. Only the rows of the call are loaded.
+    const int chunks = REREAD ? (un.p1 + W * kWarpRows - 1) / (W * kWarpRows) : 1;
+    auto row_of = [&](int q, int i) { return (q * W + wu) * kWarpRows + i * RPP + rl; };
+    Row16<T> r[PASSES];
+    auto load_rows = [&](int q) {
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int p = row_of(q, i);
+            if (col && p >= un.p0 && p < un.p1)
+                r[i].load(src + (un.row0 + (p - un.p0)) * a.src_s0[m]);
+            else
+                r[i].clear();
+        }
+    };
+    const float old = here && un.p0 > 0 ? *scale : 0.f;   // read by every lane before the barrier below, written after it
+
+    float amax = 0.f;
+    int odd = 0;   // a NaN or an infinity among the rows
+    for (int q = 0; q < chunks; ++q) {
+        load_rows(q);
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            float f[16];
+            r[i].unpack(f);
+            float mx = 0.f, chk = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                mx = fmaxf(mx, fabsf(f[e]));
+                chk = fmaf(f[e], 0.f, chk);   // NaN for a NaN or an infinity
+            }
+            if (chk != 0.f) {
+                odd = 1;
+                mx = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, isfinite(f[e]) ? fabsf(f[e]) : 0.f);
+            }
+            amax = fmaxf(amax, mx);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    odd = __any_sync(0xffffffffu, odd);
+    if constexpr (W > 1) {
+        if (lane == 0) {
+            s_amax[warp] = amax;
+            s_odd[warp] = odd;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            amax = fmaxf(amax, s_amax[warp / W * W + w]);
+            odd |= s_odd[warp / W * W + w];
+        }
+    } else {
+        __syncwarp();
+    }
+    if (!here) return;
+
+    float s = fresh_scale(amax, a.e4m3);
+    if (un.p0 > 0 && old > 0.f) {
+        const int steps = growth_steps(old, s);
+        s = steps > 0 ? static_cast<float>(scalbn(static_cast<double>(old), steps)) : old;
+        if (steps > 0) {   // what earlier calls left in this block, in the grown scale
+            const float f = pow2f(-steps);
+            for (int p = wu * kWarpRows + rl; p < un.p0; p += (p % kWarpRows + RPP < kWarpRows) ? RPP : (W - 1) * kWarpRows + RPP) {
+                if (!col) continue;
+                uint4* at = reinterpret_cast<uint4*>(dst + static_cast<int64_t>(p) * a.c_s1[m]);
+                uint4 v = *at;
+                uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t o = 0;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) o |= shrink_code((w[e] >> (8 * b)) & 0xffu, f, a.e4m3) << (8 * b);
+                    w[e] = o;
+                }
+                *at = v;
+            }
+        }
+    }
+    if (wu == 0 && lane == 0) *scale = s;
+
+    const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+    const float half_step = 0.5f * s;
+    for (int q = 0; q < chunks; ++q) {
+        if (REREAD) load_rows(q);
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int p = row_of(q, i);
+            if (!col || p < un.p0 || p >= un.p1) continue;
+            float f[16];
+            r[i].unpack(f);
+            uint32_t w[4];
+            float off = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = encode4(f + 4 * e, s, inv, a.e4m3, off);
+            if (odd || s == 0.f || (!a.e4m3 && off >= half_step)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    w[e] = 0;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) w[e] |= encode_slow(f[4 * e + b], s, a.e4m3) << (8 * b);
+                }
+            }
+            *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(p) * a.c_s1[m]) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+// Any width, strides and alignment: one CTA to a unit, element by element.
+template <typename T>
+__global__ void __launch_bounds__(kCopyThreads) quantized_copy_any_kernel(const QuantCopyArgs a) {
+    __shared__ float s_amax[kCopyWarps];
+    const int m = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+    const CopyUnit un = find_unit(a, blockIdx.x);
+    if (un.block < 0) return;
+    const T* src = static_cast<const T*>(a.src[m]) + un.row0 * a.src_s0[m] + static_cast<int64_t>(h) * a.src_s1[m];
+    uint8_t* dst = static_cast<uint8_t*>(a.cache[m]) + un.block * a.c_s0[m] + static_cast<int64_t>(h) * a.c_s2[m];
+    float* scale = a.scale[m] + un.block * a.s_s0[m] + static_cast<int64_t>(h) * a.s_s1[m];
+    const float old = un.p0 > 0 ? *scale : 0.f;
+    const int64_t n = static_cast<int64_t>(un.p1 - un.p0) * a.D;
+    float amax = 0.f;
+    for (int64_t i = tid; i < n; i += kCopyThreads) {
+        const float x = Cvt<T>::to_f(src[i / a.D * a.src_s0[m] + i % a.D * a.src_s2[m]]);
+        amax = fmaxf(amax, isfinite(x) ? fabsf(x) : 0.f);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if ((tid & 31) == 0) s_amax[tid >> 5] = amax;
+    __syncthreads();
+    for (int w = 0; w < kCopyWarps; ++w) amax = fmaxf(amax, s_amax[w]);
+    float s = fresh_scale(amax, a.e4m3);
+    if (un.p0 > 0 && old > 0.f) {
+        const int steps = growth_steps(old, s);
+        s = steps > 0 ? static_cast<float>(scalbn(static_cast<double>(old), steps)) : old;
+        if (steps > 0) {
+            const float f = pow2f(-steps);
+            for (int64_t i = tid; i < static_cast<int64_t>(un.p0) * a.D; i += kCopyThreads) {
+                uint8_t* at = dst + i / a.D * a.c_s1[m] + i % a.D * a.c_s3[m];
+                *at = static_cast<uint8_t>(shrink_code(*at, f, a.e4m3));
+            }
+        }
+    }
+    if (tid == 0) *scale = s;
+    for (int64_t i = tid; i < n; i += kCopyThreads) {
+        const float x = Cvt<T>::to_f(src[i / a.D * a.src_s0[m] + i % a.D * a.src_s2[m]]);
+        dst[(un.p0 + i / a.D) * a.c_s1[m] + i % a.D * a.c_s3[m]] = static_cast<uint8_t>(encode_slow(x, s, a.e4m3));
+    }
+}
+
+template <typename T, int LPR>
+void launch_rows(const QuantCopyArgs& a, int units, cudaStream_t st) {
+    auto go = [&](auto kern, int w) {
+        const int upc = kCopyWarps / w;
+        kern<<<dim3(units, (a.H + upc - 1) / upc, 2), kCopyThreads, 0, st>>>(a);
+    };
+    if (a.block_size <= 16) go(quantized_copy_kernel<T, LPR, 1, false>, 1);
+    else if (a.block_size <= 32) go(quantized_copy_kernel<T, LPR, 2, false>, 2);
+    else if (a.block_size <= 64) go(quantized_copy_kernel<T, LPR, 4, false>, 4);
+    else if (a.block_size <= 128) go(quantized_copy_kernel<T, LPR, 8, false>, 8);
+    else go(quantized_copy_kernel<T, LPR, 8, true>, 8);
+}
+
+template <typename T>
+void launch_t(const QuantCopyArgs& a, int units, cudaStream_t st) {
+    bool rows = a.D % 16 == 0 && a.D <= 256;
+    for (int m = 0; m < 2; ++m) {
+        rows = rows && a.src_s2[m] == 1 && (a.src_s0[m] * sizeof(T)) % 16 == 0 && (a.src_s1[m] * sizeof(T)) % 16 == 0 &&
+               reinterpret_cast<uintptr_t>(a.src[m]) % 16 == 0;
+        rows = rows && a.c_s3[m] == 1 && a.c_s0[m] % 16 == 0 && a.c_s1[m] % 16 == 0 && a.c_s2[m] % 16 == 0 &&
+               reinterpret_cast<uintptr_t>(a.cache[m]) % 16 == 0;
+    }
+    if (!rows)
+        quantized_copy_any_kernel<T><<<dim3(units, a.H, 2), kCopyThreads, 0, st>>>(a);
+    else if (a.D <= 64)
+        launch_rows<T, 4>(a, units, st);
+    else if (a.D <= 128)
+        launch_rows<T, 8>(a, units, st);
+    else
+        launch_rows<T, 16>(a, units, st);
+}
+
+}  // namespace
+
+void launch_quantized_copy_kv(const QuantCopyArgs& a, cudaStream_t st) {
+    // Touched blocks of a request of n tokens: n at most, and n / block_size + 2 at most.
+    const int64_t units = std::min<int64_t>(a.T, a.T / a.block_size + 2ll * a.B);
+    if (units <= 0) return;
+    if (a.dt == Dt::F16)
+        launch_t<__half>(a, static_cast<int>(units), st);
+    else if (a.dt == Dt::BF16)
+        launch_t<__nv_bfloat16>(a, static_cast<int>(units), st);
+    else
+        launch_t<float>(a, static_cast<int>(units), st);
+}
+
+}  // namespace k
+}  // namespace b200

@@ -112,6 +112,36 @@ def paged_attention(query, key, value, attenMask, actualSeqLengths, numHeads, nu
     return out
 
 
+def build_block_table(block_table, cached_lens, new_lens, free_blocks, free_start, block_size, *, slot_map, new_start, seq_lens, free_next, token_table=None,
+                      ctx=None, as_device=None):
+    """Blocks, slots and offsets of a batch whose requests hold cached_lens tokens and get new_lens more, on the device: takes
+    blocks from free_blocks[free_start:] in request order, writes their entries of block_table [B, cols], slot_map [T] (the
+    slot of each new token; INT32_MIN behind the last), new_start [B + 1], seq_lens [B], free_next [1] and, when given,
+    token_table [B, N] (one slot for each token, right-aligned: the b_loc of token_decode_attention). Returns block_table."""
+    ts = [_t(x, as_device) for x in (block_table, slot_map, new_start, seq_lens, token_table, free_next, cached_lens, new_lens, free_blocks, free_start)]
+    _call("diopiBuildBlockTable", ctx, *[_h(t) for t in ts], int(block_size))
+    return block_table
+
+
+def quantized_copy_kv(k, v, block_table, cached_lens, new_start, k_cache, v_cache, k_scale, v_scale, *, ctx=None, as_device=None):
+    """Rows new_start[i] + t of k, v [T, Hkv, D] into positions cached_lens[i] + t of request i of the 8-bit caches
+    [blocks, block_size, Hkv, D] (int8, or float8_e4m3fn / uint8 holding its bits), whose scales [blocks, Hkv] start anew with a
+    block and grow by powers of two after that. Returns (k_cache, v_cache)."""
+    ts = [_t(x, as_device) for x in (k_cache, v_cache, k_scale, v_scale, k, v, block_table, cached_lens, new_start)]
+    _call("diopiQuantizedCopyKV", ctx, *[_h(t) for t in ts])
+    return k_cache, v_cache
+
+
+def quantized_paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, softmax_scale, *, out=None, ctx=None, as_device=None):
+    """Attention of the newest token (q [B, H, D]) or the n newest tokens (q [B, n, H, D], causal among them) of each request
+    over the 8-bit caches; seq_lens counts all tokens, the new ones among them. Returns out (a new tensor like q)."""
+    if out is None:
+        out = torch.empty_like(q)
+    ts = [_t(x, as_device) for x in (out, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens)]
+    _call("diopiQuantizedPagedAttention", ctx, *[_h(t) for t in ts], float(softmax_scale))
+    return out
+
+
 def apply_penalty(logits, presence_penalty, frequency_penalty, p_token_ids, p_token_counts, p_cumsum_seq_len,
                   p_max_len_in_batch, *, ctx=None, as_device=None):
     """In-place presence/frequency penalty; returns logits."""

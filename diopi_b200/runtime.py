@@ -38,6 +38,7 @@ _TORCH_TO_DIOPI = {
     torch.int8: Dtype.int8, torch.uint8: Dtype.uint8, torch.int16: Dtype.int16, torch.int32: Dtype.int32,
     torch.int64: Dtype.int64, torch.float16: Dtype.float16, torch.float32: Dtype.float32,
     torch.float64: Dtype.float64, torch.bool: Dtype.bool, torch.bfloat16: Dtype.bfloat16,
+    torch.float8_e4m3fn: Dtype.uint8,   # the interface has no 8-bit float: ops that take e4m3 take its bits as uint8
 }
 
 SUCCESS, ERROR_OCCURRED, NO_IMPLEMENT, DTYPE_NOT_SUPPORTED = 0, 1, 13, 1000

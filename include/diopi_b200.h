@@ -237,6 +237,48 @@ diopiError_t diopiRotaryEmbeddingCopyKV(diopiContextHandle_t ctx, diopiTensorHan
                                         diopiConstTensorHandle_t q, diopiConstTensorHandle_t k, diopiConstTensorHandle_t v, diopiConstTensorHandle_t cos,
                                         diopiConstTensorHandle_t sin, diopiConstTensorHandle_t dest_loc, bool conj);
 
+/* Extensions (not in the DIOPI headers): serving from a block-paged K/V cache held in 8 bits. The block size is that of
+ * diopiPagedAttention's block_table (functions_ext.h:616-618), and slots count block * block_size + position, as there.
+ *
+ * diopiBuildBlockTable: from the lengths of a batch, on the device. Request i holds cached_lens[i] tokens and gets
+ * new_lens[i] more; the blocks it still needs are taken from free_blocks [n_free] in request order, the first at
+ * free_start [1]. Written: the taken blocks' entries of block_table [B, cols] (entries of blocks already held are read, the
+ * others stay as they were); slot_map [T]: the slot of every new token, packed by request; new_start [B+1]: where each
+ * request's new tokens begin; seq_lens [B] = cached + new; free_next [1] = free_start + blocks taken; and, unless it is
+ * null, token_table [B, N]: the slot of every token of request i, right-aligned (the b_loc of the ops above; columns in
+ * front of a request's first token stay as they were). Index tensors are int32 or int64 each. No output may overlap an
+ * input or another output, except that block_table is both.
+ * Entries of slot_map behind the last new token are INT32_MIN, which every op of this library skips. When the free list
+ * runs out or a request outgrows its row, the missing blocks get the entry -1 and their tokens the slot INT32_MIN, tokens
+ * beyond the row are not counted in seq_lens, and the next call on the device reports it (status 4). */
+diopiError_t diopiBuildBlockTable(diopiContextHandle_t ctx, diopiTensorHandle_t block_table, diopiTensorHandle_t slot_map, diopiTensorHandle_t new_start,
+                                  diopiTensorHandle_t seq_lens, diopiTensorHandle_t token_table, diopiTensorHandle_t free_next,
+                                  diopiConstTensorHandle_t cached_lens, diopiConstTensorHandle_t new_lens, diopiConstTensorHandle_t free_blocks,
+                                  diopiConstTensorHandle_t free_start, int64_t block_size);
+
+/* diopiQuantizedCopyKV: writes new rows k, v [T, Hkv, D] (fp16, bf16, fp32) into k_cache, v_cache [blocks, block_size, Hkv, D]
+ * and their scales k_scale, v_scale [blocks, Hkv] (float32). The caches are int8, or uint8 holding the bits of e4m3
+ * values; a code c in a block with scale s stands for c * s. Row new_start[i] + t is the token at position
+ * cached_lens[i] + t of request i; rows behind new_start[B] are not read. A block whose position 0 is written begins anew:
+ * s = amax / 127 in fp32 (int8), the smallest power of two with amax <= 448 s (e4m3), 2^-126 at least, 0 when amax = 0,
+ * with amax the largest finite magnitude of the call's rows in it. A block that holds earlier tokens keeps s, or grows it
+ * by the smallest sufficient power of two and rounds the codes in front of the new rows to the grown scale. Codes are the
+ * nearest to x / s, ties to even; infinities saturate, NaN becomes 0 (int8) or NaN (e4m3). Positions behind the new
+ * rows stay as they were. Two requests must not write one block in the same call; rows whose block is
+ * outside the cache are skipped (status 1). */
+diopiError_t diopiQuantizedCopyKV(diopiContextHandle_t ctx, diopiTensorHandle_t k_cache, diopiTensorHandle_t v_cache, diopiTensorHandle_t k_scale,
+                                  diopiTensorHandle_t v_scale, diopiConstTensorHandle_t k, diopiConstTensorHandle_t v, diopiConstTensorHandle_t block_table,
+                                  diopiConstTensorHandle_t cached_lens, diopiConstTensorHandle_t new_start);
+
+/* diopiQuantizedPagedAttention: decode attention over such a cache. q, out [B, H, D] or [B, n, H, D] (fp16, bf16, fp32;
+ * H a multiple of Hkv): the n newest tokens of each request, whose K/V rows are in the cache already. seq_lens [B] counts
+ * all tokens of a request; token t of n sees the first seq_lens[i] - (n - 1 - t) of them, causally, and one that sees none
+ * gets zeros. out = softmax(softmax_scale * q k^T) v with softmax_scale > 0. Scales must not be negative. Tokens in a block
+ * outside the cache are left out (status 1). */
+diopiError_t diopiQuantizedPagedAttention(diopiContextHandle_t ctx, diopiTensorHandle_t out, diopiConstTensorHandle_t q, diopiConstTensorHandle_t k_cache,
+                                          diopiConstTensorHandle_t v_cache, diopiConstTensorHandle_t k_scale, diopiConstTensorHandle_t v_scale,
+                                          diopiConstTensorHandle_t block_table, diopiConstTensorHandle_t seq_lens, double softmax_scale);
+
 /* out [.., N] = sum over the ranks of `group` of (x1 [.., K] @ x2 [K, N] + bias [N]): the row-parallel linear layer of a
  * tensor-parallel model as one kernel per rank (tcgen05 GEMM whose epilogue stores the fp32 partial tiles into every
  * rank's staging area over NVLink; each rank then adds the partials in rank order, so all ranks hold identical bits).
