@@ -1,7 +1,7 @@
 // New K and V rows into a paged cache of 8-bit codes with one scale for each (block, head) (diopiQuantizedCopyKV).
 //
 // A block whose first position is written by the call begins anew: with amax the largest magnitude of the call's rows in it
-//     int8:  s = max(fp32(amax / 127), 2^-126)         e4m3:  s = 2^k, the smallest k >= -126 with amax <= 448 * 2^k
+//     int8:  s = max(amax * fp32(1 / 127), 2^-126)         e4m3:  s = 2^k, the smallest k >= -126 with amax <= 448 * 2^k
 // (s = 0 when amax = 0). A block that an earlier call began keeps its tokens: its scale becomes s' = s * 2^k with the
 // smallest k >= 0 that covers the new rows, and the codes in front of them become rne(code * 2^-k). Growth by powers of two
 // keeps that exact where the format can hold the result, so that a block filled token by token does not drift. A new code is
@@ -30,7 +30,7 @@ constexpr float kFltMin = 1.17549435e-38f;   // 2^-126
 // The scale of a block that begins anew.
 __device__ __forceinline__ float fresh_scale(float amax, bool e4m3) {
     if (!(amax > 0.f)) return 0.f;
-    if (!e4m3) return fmaxf(__fdiv_rn(amax, 127.f), kFltMin);
+    if (!e4m3) return fmaxf(__fmul_rn(amax, 1.f / 127.f), kFltMin);
     const uint32_t u = __float_as_uint(amax);
     const int e = static_cast<int>(u >> 23);                       // biased; 0 for subnormals
     int k = e - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);         // 448 = 1.75 * 2^8

@@ -260,7 +260,7 @@ diopiError_t diopiBuildBlockTable(diopiContextHandle_t ctx, diopiTensorHandle_t 
  * and their scales k_scale, v_scale [blocks, Hkv] (float32). The caches are int8, or uint8 holding the bits of e4m3
  * values; a code c in a block with scale s stands for c * s. Row new_start[i] + t is the token at position
  * cached_lens[i] + t of request i; rows behind new_start[B] are not read. A block whose position 0 is written begins anew:
- * s = amax / 127 in fp32 (int8), the smallest power of two with amax <= 448 s (e4m3), 2^-126 at least, 0 when amax = 0,
+ * s = amax * (1 / 127), both roundings in fp32 (int8), the smallest power of two with amax <= 448 s (e4m3), 2^-126 at least, 0 when amax = 0,
  * with amax the largest finite magnitude of the call's rows in it. A block that holds earlier tokens keeps s, or grows it
  * by the smallest sufficient power of two and rounds the codes in front of the new rows to the grown scale. Codes are the
  * nearest to x / s, ties to even; infinities saturate, NaN becomes 0 (int8) or NaN (e4m3). Positions behind the new

@@ -48,7 +48,7 @@ def fresh_scale(amax: float, e4m3: bool) -> float:
     if not amax > 0:
         return 0.0
     if not e4m3:
-        return max(float(torch.tensor(amax, dtype=torch.float32) / torch.tensor(127.0, dtype=torch.float32)), 2.0 ** -126)
+        return max(float(torch.tensor(amax, dtype=torch.float32) * torch.tensor(1 / 127, dtype=torch.float32)), 2.0 ** -126)
     k = -126
     while amax > 448.0 * 2.0 ** k:
         k += 1
@@ -114,11 +114,12 @@ def quantized_copy(x, block_table, cached, new_start, cache, scale):
 
 
 def quantized_paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, softmax_scale):
-    """q [B, n, H, D]. Returns (out, weight, logit) in fp64, shaped like q, [B, n, H, D] and [B, n, H]: the result, the same sum with
-    |v| in the place of v, and the largest softmax_scale * sum |q| |k|, which error bounds go by."""
+    """q [B, n, H, D]. Returns (out, (weight, reach, logit)) in fp64: the result, and what error bounds go by: the same sum with |v|
+    in the place of v, the sum of |v| alone (both [B, n, H, D]), and the largest softmax_scale * sum |q| |k| ([B, n, H])."""
     B, n, H, D = q.shape
     bs, Hkv = k_cache.shape[1], k_cache.shape[2]
-    out, weight, logit = torch.zeros(B, n, H, D, dtype=torch.float64), torch.zeros(B, n, H, D, dtype=torch.float64), torch.zeros(B, n, H, dtype=torch.float64)
+    out, weight, reach = [torch.zeros(B, n, H, D, dtype=torch.float64) for _ in range(3)]
+    logit = torch.zeros(B, n, H, dtype=torch.float64)
     for i, L in enumerate(seq_lens.tolist()):
         L = min(max(L, 0), block_table.shape[1] * bs)
         pos = torch.arange(L)
@@ -137,5 +138,6 @@ def quantized_paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table
                     p = torch.softmax(x, 0)
                     out[i, t, g] = p @ v[see]
                     weight[i, t, g] = p @ v[see].abs()
+                    reach[i, t, g] = v[see].abs().sum(0)
                     logit[i, t, g] = (softmax_scale * (k[see].abs() @ q[i, t, g].double().abs())).max()
-    return out, weight, logit
+    return out, (weight, reach, logit)
