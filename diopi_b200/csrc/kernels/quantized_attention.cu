@@ -4,23 +4,22 @@
 // New token t of n sees the first L - (n - 1 - t) tokens; a row that sees none gives zeros.
 //
 // quant_split_kernel (block_size and head_dim multiples of 16, head_dim up to 256) is bound by the bytes of the codes. The
-// query rows that share a K/V head (n * group of them) are the M extent of mma.sync m16n8k16 in fp16 with fp32
-// accumulators, as in token_decode_gqa.cu: every code of either kind is an fp16 number, so nothing is lost by the
-// conversion in registers, and the scales stay outside the products. A tile is 16 tokens of one K/V head, always inside one
-// block, hence one ks and one vs:
-//     S = Q Kc^T;  m = max(S * f), f = ks * softmax_scale * log2 e;  P = 2^(S f - m + 15);  O += (2^(m - ref) vs) (P Vc)
+// query rows that share a K/V head (n * group of them) are the N extent of mma.sync m16n8k16 in fp16 with fp32
+// accumulators: every code of either kind is an fp16 number, so nothing is lost by the conversion in registers, and the
+// scales stay outside the products. A tile is 16 tokens of one K/V head, always inside one block, hence one ks and one vs:
+//     S^T = Kc Q^T;  m = max(S f), f = ks * softmax_scale * log2 e;  P = 2^(S f - m + 15);  O^T += (2^(m - ref) vs) (Vc^T P^T)
 // The weights are taken against the tile's own maximum, so that they fill fp16's range (2^15 down to 2^-24: what is lost is
-// below 2^-40 of the tile's largest weight) whatever the other tiles hold, and the
-// product of a tile is added in fp32 with its factor; ref is only raised when a tile exceeds it by 2^40. Queries are scaled
-// by the power of two that brings their row's maximum to [1, 2) before they become fp16 (bf16 and fp32 reach further than
-// fp16 does); fp32 queries and their weights are split into two fp16 numbers each, with two products.
+// below 2^-40 of the tile's largest weight) whatever the other tiles hold, and the product of a tile is added in fp32 with
+// its factor; ref is only raised when a tile exceeds it by 2^40. Queries are scaled by the power of two that brings their
+// row's maximum to [1, 2) before they become fp16 (bf16 and fp32 reach further than fp16 does); fp32 queries and their
+// weights are split into two fp16 numbers each, with two products.
 //
-// Work split: a step is TT tokens of hw K/V heads; the steps of the batch are cut into equal ranges, one per CTA, and the parts of a
-// request that fell to several CTAs are merged by quant_combine_kernel (a programmatic dependent launch). A request that
-// one CTA has whole is written by it directly. Eight consumer warps are (token tile, M tile, K/V head); one producer warp
-// looks up the blocks two batches of steps ahead and their scales one ahead, and fetches a tile of hw heads with one TMA
-// load each for K and V ([head][token][128 bytes], swizzled: the reads below are free of bank conflicts whatever the layout of
-// the cache in memory).
+// Work split: the tiles of the batch are cut into equal ranges, one per team, a team being the warps of one K/V head (one warp for up
+// to 8 * NT query rows, mt of them beyond). The teams of a CTA are hw neighbouring heads of the same range, which keeps their reads
+// next to each other in memory, times tw ranges. A team has a ring of tiles of its own, filled by TMA (two loads, K and V, of 16 rows,
+// swizzled: the reads below are free of bank conflicts), and its leader refills a slot as soon as it is read: no producer warp, and no
+// barrier between teams. Block ids and scales of the next 32 tiles are held by the 32 lanes. Where a request falls into several
+// ranges its parts are merged by quant_combine_kernel (a programmatic dependent launch); else it is written directly.
 //
 // quant_plain_kernel: any width, strides and block size; one CTA to a query row, a warp to every fourth token.
 #include <cuda.h>
@@ -128,25 +127,26 @@ __global__ void __launch_bounds__(32 * kPlainWarps) quant_plain_kernel(const Qua
 // ---------------------------------------------------------------------------------------------------
 // The split kernel.
 // ---------------------------------------------------------------------------------------------------
-constexpr int kQWarps = 8;                      // consumer warps
-constexpr int kQThreads = 32 * (kQWarps + 1);
-constexpr int kQMaxStages = 16;
+constexpr int kQMaxStages = 8;
 constexpr int kQMaxB = 4096;
 constexpr int kTile = 16;                       // tokens of a tile
-constexpr int kStepsPerCta = 2;                 // a CTA gets this many steps at least, so that short batches are not cut into crumbs
+constexpr int kTilesPerRange = 4;               // at least, so that short batches are not cut into crumbs
+
+// Warps of a CTA: as many as the registers of a thread's queries and accumulators leave room for (a spilled register costs
+// an L2 access here, as shared memory leaves no L1).
+constexpr int split_warps(bool f32, int hd, int nt) { return hd > 128 || nt > 1 ? 8 : f32 ? 12 : 16; }
 
 struct QuantPlan {
     int hd;           // 64, 128 or 256: head_dim rounded up
+    int nt;           // N tiles of 8 query rows of a warp
+    int mt;           // warps of a team
+    int n_z;          // CTAs along the query rows of a K/V head
     int hw;           // K/V heads of a CTA: a divisor of Hkv
     int n_hg;         // CTAs along the K/V heads
-    int mt;           // M tiles of 16 query rows of a CTA
-    int n_z;          // CTAs along the query rows of a K/V head (more than 128 of them)
-    int tw;           // token tiles that the warps work on side by side
-    int ts;           // token tiles that a warp works through in one step
-    int tt;           // tokens of a step: 16 * tw * ts
-    int items;        // (tile, head) pairs of a step: hw * tw * ts, at most 16
-    int stage_bytes, nstages, n_cta;
-    int off_meta, off_bars, off_pre, off_len, off_red, off_flag, smem_bytes;
+    int tw;           // ranges of a CTA
+    int stages;       // tiles of a team's ring
+    int n_cta, n_range;
+    int off_bars, off_pre, off_len, off_flag, smem_bytes;
     bool qvec;        // four elements of q can be loaded at once
 };
 
@@ -166,6 +166,12 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+// 8 x 8 transpose of 16-bit elements: lane 4 r + c holds columns 2c, 2c + 1 of row r, before and after.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 // What two fp32 values lose as fp16, as fp16.
 __device__ __forceinline__ uint32_t pack_rest(float lo, float hi, uint32_t packed) {
@@ -188,55 +194,26 @@ __device__ __forceinline__ void codes_to_f16(uint32_t c, uint32_t& lo, uint32_t&
     }
 }
 
-// Steps [t, t1) of the flattened (request, step) pairs.
-struct QuantWalk {
-    const int* pre;   // pre[i] = first step of request i
-    int t, t1, i;
-    __device__ void init(const int* pre_, int B, int t0_, int t1_) {
-        pre = pre_;
-        t = t0_;
-        t1 = t1_;
-        int lo = 0, hi = B;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (pre[mid + 1] > t)
-                hi = mid;
-            else
-                lo = mid + 1;
-        }
-        i = lo;
-    }
-    __device__ bool next(int& req, int& step, bool& last) {
-        if (t >= t1) return false;
-        while (pre[i + 1] <= t) ++i;
-        req = i;
-        step = t - pre[i];
-        ++t;
-        last = t == t1 || t == pre[i + 1];
-        return true;
-    }
-};
+__device__ __forceinline__ int used_ranges(int total, int n_range) { return max(1, min(n_range, (total + kTilesPerRange - 1) / kTilesPerRange)); }
 
-__device__ __forceinline__ int used_ctas(int total, int n_cta) { return max(1, min(n_cta, (total + kStepsPerCta - 1) / kStepsPerCta)); }
-
-template <typename T, bool E4M3, int HD>
-__global__ void __launch_bounds__(kQThreads, 1)
+template <typename T, bool E4M3, int HD, int NT>
+__global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value, HD, NT), 1)
     quant_split_kernel(const QuantAttnArgs a, const QuantPlan p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        float* __restrict__ ws_acc, float* __restrict__ ws_ml) {
     constexpr bool SPLIT = std::is_same<T, float>::value;   // two fp16 numbers for each fp32 one
     constexpr int RB = HD < 128 ? HD : 128;                 // bytes of a row of one TMA box
     constexpr int NH = HD / RB;                             // boxes side by side (head_dim 256: 2)
-    constexpr int CH = HD / 16;                             // k steps of Q K^T: 16 bytes of codes each
+    constexpr int CH = HD / 16;                             // k steps of Kc Q^T: 16 bytes of codes each
     constexpr int VB = RB / 8;                              // bytes of a V row that a lane takes from each box
-    constexpr int DN = HD / 8;                              // n tiles of P V
-    constexpr int HEAD_TILE = kTile * RB;                   // bytes of one head's tile in a box
+    constexpr int DM = HD / 16;                             // M tiles of Vc^T P^T
+    constexpr int BOX = kTile * RB;                         // bytes of a box
+    constexpr uint32_t STAGE = 2 * NH * BOX;                // K, then V
+    constexpr int kThreads = 32 * split_warps(SPLIT, HD, NT);
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the swizzle goes by address bits
-    float4* meta = reinterpret_cast<float4*>(smem + p.off_meta);                          // [stage][item]: ks, vs, tokens
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.off_bars);                      // full[nstages], empty[nstages], merge[2]
-    int* pre = reinterpret_cast<int*>(smem + p.off_pre);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.off_bars);                      // [team][full, empty][stage]
+    int* pre = reinterpret_cast<int*>(smem + p.off_pre);                                  // pre[i] = first tile of request i
     int* lens = reinterpret_cast<int*>(smem + p.off_len);
-    float* red = reinterpret_cast<float*>(smem + p.off_red);
     volatile int* give_up = reinterpret_cast<volatile int*>(smem + p.off_flag);
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -244,24 +221,22 @@ __global__ void __launch_bounds__(kQThreads, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = a.Hq / a.Hkv;
     const int R = a.n * group;                 // query rows of a K/V head
-    const int hg0 = blockIdx.y * p.hw;
-    const int active = p.hw * p.mt * p.tw;     // consumer warps with work
+    const int teams = p.hw * p.tw;
 
+    if (tid < teams * p.stages) {
+        uint64_t* b = bars + tid / p.stages * (2 * p.stages) + tid % p.stages;
+        mbar_init(smem_u32(b), 1);
+        mbar_init(smem_u32(b + p.stages), p.mt);
+    }
     if (tid == 0) {
-        for (int s = 0; s < p.nstages; ++s) {
-            mbar_init(smem_u32(&bars[s]), 1);
-            mbar_init(smem_u32(&bars[p.nstages + s]), active);
-        }
-        mbar_init(smem_u32(&bars[2 * p.nstages]), active);
-        mbar_init(smem_u32(&bars[2 * p.nstages + 1]), active);
         *give_up = 0;
         pre[0] = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    for (int i = tid; i < a.B; i += kQThreads) {
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    for (int i = tid; i < a.B; i += kThreads) {
         const int L = quant_len(a, i);
         lens[i] = L;
-        pre[i + 1] = (L + p.tt - 1) / p.tt;
+        pre[i + 1] = (L + kTile - 1) / kTile;
     }
     __syncthreads();
     if (warp == 0) {
@@ -280,173 +255,146 @@ __global__ void __launch_bounds__(kQThreads, 1)
     }
     __syncthreads();
 
+    const int team = warp / p.mt, mtile = warp - team * p.mt;
+    const int hl = team % p.hw, range = blockIdx.x * p.tw + team / p.hw;
     const int total = pre[a.B];
-    const int used = used_ctas(total, p.n_cta), cta = blockIdx.x;
-    if (cta >= used) return;
-    const int t0 = static_cast<int>(static_cast<int64_t>(total) * cta / used);
-    const int t1 = static_cast<int>(static_cast<int64_t>(total) * (cta + 1) / used);
-    const uint32_t ring0 = smem_u32(smem);
-    const uint32_t box_bytes = static_cast<uint32_t>(p.hw) * HEAD_TILE;
-    const uint32_t tiles = static_cast<uint32_t>(p.tw * p.ts);
-    const uint32_t v_off = tiles * NH * box_bytes;
+    const int used = used_ranges(total, p.n_range);
+    if (team < teams && range < used) {
+        const int t0 = static_cast<int>(static_cast<int64_t>(total) * range / used);
+        const int t1 = static_cast<int>(static_cast<int64_t>(total) * (range + 1) / used);
+        const int hkv = blockIdx.y * p.hw + hl;
+        const uint32_t ring0 = smem_u32(smem) + static_cast<uint32_t>(team * p.stages) * STAGE;
+        const uint32_t full0 = smem_u32(bars + team * 2 * p.stages), empty0 = full0 + 8u * p.stages;
 
-    if (warp == kQWarps) {
-        // =========================== producer warp ===============================
-        // A lane is one (token tile, head) pair of one of the next 32 / items steps. Three batches of steps are on their way:
-        // the block ids of one are being loaded, the scales of the one before, and the one before that is issued.
-        const int per_batch = 32 / p.items;
-        const int sb = lane / p.items, item = lane - sb * p.items;
-        const int tile = item / p.hw, hl = item - tile * p.hw;
-        struct Batch {
-            int n = 0, valid = 0, at = 0;
-            int64_t block = -1;
-            float ks = 0.f, vs = 0.f;
-        } cur, nxt, far;
-        QuantWalk walk;
-        walk.init(pre, a.B, t0, t1);
-        auto load_ids = [&](Batch& b) {
-            int req = 0, step = 0, my_req = -1, my_step = 0;
-            bool last;
-            b.n = 0;
-            for (; b.n < per_batch; ++b.n) {
-                if (!walk.next(req, step, last)) break;
-                if (b.n == sb) {
-                    my_req = req;
-                    my_step = step;
-                }
+        // ---- what the lanes know of 32 tiles: lane k of tile base + k ----
+        struct Ahead {
+            int block, at;   // at = 32 * position in the block + tokens (0: leave the tile out)
+            float ks, vs;
+        } cur, nxt;
+        auto request_of = [&](int t) {
+            int lo = 0, hi = a.B;   // smallest i with pre[i + 1] > t
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (pre[mid + 1] > t)
+                    hi = mid;
+                else
+                    lo = mid + 1;
             }
-            b.valid = 0;
-            if (my_req >= 0) {
-                const int pos = my_step * p.tt + tile * kTile;
-                b.valid = max(0, min(kTile, lens[my_req] - pos));
-                if (b.valid > 0) {
-                    const int col = pos / a.block_size;
-                    b.at = pos - col * a.block_size;
-                    b.block = load_index(a.table, my_req, col);
-                }
+            return lo;
+        };
+        auto load_ids = [&](Ahead& x, int base) {
+            x.block = 0;
+            x.at = 0;
+            x.ks = x.vs = 0.f;
+            const int t = base + lane;
+            if (t < t1) {
+                const int i = request_of(t);
+                const int pos = (t - pre[i]) * kTile, col = pos / a.block_size;
+                const int64_t id = load_index(a.table, i, col);
+                const bool ok = id >= 0 && id < a.blocks;
+                if (!ok) report_status(a.status, 1);
+                x.block = ok ? static_cast<int>(id) : 0;
+                x.at = ok ? (pos - col * a.block_size) * 32 + min(kTile, lens[i] - pos) : 0;
             }
         };
-        auto load_scales = [&](Batch& b) {
-            if (b.valid > 0) {
-                if (b.block < 0 || b.block >= a.blocks) {
-                    report_status(a.status, 1);
-                    b.valid = 0;
-                } else {
-                    b.ks = a.scale[0][b.block * a.s_s0[0] + static_cast<int64_t>(hg0 + hl) * a.s_s1[0]];
-                    b.vs = a.scale[1][b.block * a.s_s0[1] + static_cast<int64_t>(hg0 + hl) * a.s_s1[1]];
-                }
+        auto load_scales = [&](Ahead& x) {
+            if (x.at != 0) {
+                x.ks = a.scale[0][x.block * a.s_s0[0] + hkv * a.s_s1[0]];
+                x.vs = a.scale[1][x.block * a.s_s0[1] + hkv * a.s_s1[1]];
             }
         };
-        load_ids(nxt);
-        load_ids(far);
-        load_scales(nxt);
-        int ring = 0;
-        uint32_t phase = 0;
-        bool ok = true;
-        while (ok && nxt.n > 0) {
-            cur = nxt;
-            nxt = far;
-            load_ids(far);
-            load_scales(nxt);
-            for (int s = 0; s < cur.n; ++s) {
-                const uint32_t full = smem_u32(&bars[ring]);
-                const bool mine = sb == s, load = mine && hl == 0 && cur.valid > 0;
-                const uint32_t n_load = __popc(__ballot_sync(0xffffffffu, load));
-                if (lane == 0) ok = mbar_wait(smem_u32(&bars[p.nstages + ring]), phase ^ 1u, give_up);
-                ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
-                if (!ok) break;
-                if (mine) meta[ring * p.items + item] = make_float4(cur.ks, cur.vs, static_cast<float>(cur.valid), 0.f);
-                __syncwarp();
-                if (lane == 0) mbar_arrive_expect_tx(full, n_load * 2u * NH * box_bytes);
-                __syncwarp();
-                if (load) {
-                    const uint32_t dst = ring0 + static_cast<uint32_t>(ring) * p.stage_bytes + static_cast<uint32_t>(tile) * NH * box_bytes;
+        auto fetch = [&](int slot, int block, int at) {   // one lane
+            const uint32_t full = full0 + 8u * slot, dst = ring0 + slot * STAGE;
+            if (at == 0) {
+                mbar_arrive(full);
+                return;
+            }
+            mbar_arrive_expect_tx(full, STAGE);
 #pragma unroll
-                    for (int h = 0; h < NH; ++h) {
-                        tma_4d(dst + h * box_bytes, &map_k, h * RB, cur.at, hg0, static_cast<int>(cur.block), full);
-                        tma_4d(dst + v_off + h * box_bytes, &map_v, h * RB, cur.at, hg0, static_cast<int>(cur.block), full);
-                    }
-                }
-                if (++ring == p.nstages) {
-                    ring = 0;
-                    phase ^= 1u;
-                }
+            for (int h = 0; h < NH; ++h) {
+                tma_4d(dst + h * BOX, &map_k, h * RB, at >> 5, hkv, block, full);
+                tma_4d(dst + (NH + h) * BOX, &map_v, h * RB, at >> 5, hkv, block, full);
+            }
+        };
+        int base = t0;
+        load_ids(cur, base);
+        load_scales(cur);
+        if (mtile == 0) {
+            for (int k = 0; k < min(p.stages, t1 - t0); ++k) {
+                const int block = __shfl_sync(0xffffffffu, cur.block, k), at = __shfl_sync(0xffffffffu, cur.at, k);
+                if (lane == 0) fetch(k, block, at);
             }
         }
-    } else if (warp < active) {
-        // =========================== consumer warps ==============================
-        const int hl = warp % p.hw, mtile = (warp / p.hw) % p.mt, tok = warp / (p.hw * p.mt);
-        const int hkv = hg0 + hl;
+        load_ids(nxt, base + 32);
+
         const int g = lane >> 2, c = lane & 3;
-        const int r0 = (blockIdx.z * p.mt + mtile) * 16 + g, r1 = r0 + 8;   // the two query rows of this thread's accumulators
-        const int tq0 = r0 / group, tq1 = r1 / group;                       // their new tokens
-        const int64_t row0 = static_cast<int64_t>(tq0) * a.Hq + hkv * group + (r0 - tq0 * group);
-        const int64_t row1 = static_cast<int64_t>(tq1) * a.Hq + hkv * group + (r1 - tq1 * group);
+        const int rbase = (blockIdx.z * p.mt + mtile) * 8 * NT;   // first query row of this warp
         // K: lane l names row l & 7 of matrix l >> 3, matrix m being the 16 bytes 4 i + m of eight tokens. In each register the lane
         // then has four neighbouring codes of token g: k columns 2c, 2c + 1 and 2c + 8, 2c + 9 of a k step stand for d = 4c .. 4c + 3.
         const int krow = lane & 7, ksw = RB == 128 ? krow : (krow >> 1);
-        // V: the lane has VB neighbouring codes, at d = VB * g, of tokens 2c, 2c + 1, 2c + 8, 2c + 9: the k rows that its B fragments
-        // want. Column g of n tile j stands for d = VB * g + j.
-        const uint32_t v_lane = RB == 128 ? static_cast<uint32_t>(2 * c * 128) : static_cast<uint32_t>(2 * c * 64);
+        // V: the lane has VB neighbouring codes, at d = VB * g, of tokens 2c, 2c + 1, 2c + 8, 2c + 9: the k columns that its A
+        // fragments want. Rows g and g + 8 of M tile j stand for d = VB * g + 2 j and the next one.
+        const uint32_t v_lane = static_cast<uint32_t>(NH * BOX + 2 * c * RB);
 
-        uint32_t qf[CH][4], ql[SPLIT ? CH : 1][4];
-        float o[DN][4];
-        float ref0 = -INFINITY, ref1 = -INFINITY, l0 = 0.f, l1 = 0.f, rs0 = 0.f, rs1 = 0.f;
-        int cur_req = -1, part_first = 0, lim0 = 0, lim1 = 0, lim_min = 0;
-        uint32_t merge_phase = 0;
-
-        QuantWalk walk;
-        walk.init(pre, a.B, t0, t1);
-        int req, step;
-        bool last;
-        int ring = 0;
+        uint32_t qf[NT][CH][2], ql[NT][SPLIT ? CH : 1][2];
+        float o[NT][DM][4];                             // rows 2c (elements 0, 2) and 2c + 1 (1, 3) of the N tile
+        float ref[NT][2], l[NT][2], rs[NT][2];
+        int req = request_of(t0) - 1, req_end = t0, part_first = 0, lim_min = 0;
+        int slot = 0;
         uint32_t phase = 0;
-        while (walk.next(req, step, last)) {
-            if (req != cur_req) {
-                cur_req = req;
-                part_first = step;
-                ref0 = ref1 = -INFINITY;
-                l0 = l1 = 0.f;
+        for (int t = t0; t < t1; ++t) {
+            int k = t - base;
+            if (k == 32) {
+                cur = nxt;
+                base += 32;
+                k = 0;
+                load_ids(nxt, base + 32);
+            }
+            if (k == 16) load_scales(nxt);
+            if (t == req_end) {
+                do ++req;
+                while (pre[req + 1] <= t);
+                req_end = min(pre[req + 1], t1);
+                part_first = t - pre[req];
+                lim_min = lens[req] - (a.n - 1);            // what the first new token sees
 #pragma unroll
-                for (int j = 0; j < DN; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-                const int L = lens[req];
-                lim_min = L - (a.n - 1);            // what the first new token sees
-                lim0 = lim_min + tq0;
-                lim1 = lim_min + tq1;
-                // ---- the query rows as A fragments ----
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int r = half ? r1 : r0;
-                    const int tq = half ? tq1 : tq0;
+                for (int n = 0; n < NT; ++n) {
+                    // ---- query row g of the N tile as a B fragment ----
+                    const int r = rbase + 8 * n + g, tq = r / group;
                     const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(req) * a.q_s0 + static_cast<int64_t>(tq) * a.q_s1 +
-                                 static_cast<int64_t>(hkv * group + (r - tq * group)) * a.q_s2;
+                                 static_cast<int64_t>(hkv * group + (r - tq * group)) * a.q_s2 + 4 * c;
+                    const int dmax = r < R ? a.D - 4 * c : 0;
                     float amax = 0.f, scale = 1.f, back = 1.f;
-                    float x[CH][4];
+                    if constexpr (SPLIT) {
 #pragma unroll
-                    for (int k = 0; k < CH; ++k) {
-                        const int d = 16 * k + 4 * c;
-                        x[k][0] = x[k][1] = x[k][2] = x[k][3] = 0.f;
-                        if (r < R && d < a.D) {
-                            if (p.qvec) {
-                                if constexpr (SPLIT) {
-                                    const float4 v = *reinterpret_cast<const float4*>(q + d);
-                                    x[k][0] = v.x;
-                                    x[k][1] = v.y;
-                                    x[k][2] = v.z;
-                                    x[k][3] = v.w;
-                                } else {
-                                    const uint2 v = *reinterpret_cast<const uint2*>(q + d);
-                                    const T* e = reinterpret_cast<const T*>(&v);
+                        for (int i = 0; i < CH; ++i) {
+                            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (16 * i < dmax) v = p.qvec ? *reinterpret_cast<const float4*>(q + 16 * i) : make_float4(q[16 * i], q[16 * i + 1], q[16 * i + 2], q[16 * i + 3]);
+                            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+                            qf[n][i][0] = __float_as_uint(v.x);
+                            qf[n][i][1] = __float_as_uint(v.y);
+                            ql[n][i][0] = __float_as_uint(v.z);
+                            ql[n][i][1] = __float_as_uint(v.w);
+                        }
+                    } else {
 #pragma unroll
-                                    for (int i = 0; i < 4; ++i) x[k][i] = Cvt<T>::to_f(e[i]);
-                                }
-                            } else {
+                        for (int i = 0; i < CH; ++i) {
+                            uint2 v = make_uint2(0u, 0u);
+                            if (16 * i < dmax) {
+                                const unsigned short* e = reinterpret_cast<const unsigned short*>(q + 16 * i);
+                                if (p.qvec)
+                                    v = *reinterpret_cast<const uint2*>(e);
+                                else
+                                    v = make_uint2(e[0] | (static_cast<uint32_t>(e[1]) << 16), e[2] | (static_cast<uint32_t>(e[3]) << 16));
+                            }
+                            qf[n][i][0] = v.x;
+                            qf[n][i][1] = v.y;
+                            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) x[k][i] = Cvt<T>::to_f(q[d + i]);
+                                for (int h = 0; h < 2; ++h)
+                                    amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(qf[n][i][h] << 16)), fabsf(__uint_as_float(qf[n][i][h] & 0xffff0000u))));
                             }
                         }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(x[k][i]));
                     }
                     if constexpr (!std::is_same<T, __half>::value) {   // 2^-e with the row's maximum in [2^e, 2^(e + 1))
                         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
@@ -454,114 +402,120 @@ __global__ void __launch_bounds__(kQThreads, 1)
                         const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
                         scale = __uint_as_float((254u - e) << 23);
                         back = __uint_as_float(e << 23);
-                    }
 #pragma unroll
-                    for (int k = 0; k < CH; ++k) {
+                        for (int i = 0; i < CH; ++i) {
+                            if constexpr (SPLIT) {
+                                const float x0 = __uint_as_float(qf[n][i][0]) * scale, x1 = __uint_as_float(qf[n][i][1]) * scale;
+                                const float x2 = __uint_as_float(ql[n][i][0]) * scale, x3 = __uint_as_float(ql[n][i][1]) * scale;
+                                qf[n][i][0] = pack_f16(x0, x1);
+                                qf[n][i][1] = pack_f16(x2, x3);
+                                ql[n][i][0] = pack_rest(x0, x1, qf[n][i][0]);
+                                ql[n][i][1] = pack_rest(x2, x3, qf[n][i][1]);
+                            } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) x[k][i] *= scale;
-                        qf[k][half] = pack_f16(x[k][0], x[k][1]);
-                        qf[k][half + 2] = pack_f16(x[k][2], x[k][3]);
-                        if constexpr (SPLIT) {
-                            ql[k][half] = pack_rest(x[k][0], x[k][1], qf[k][half]);
-                            ql[k][half + 2] = pack_rest(x[k][2], x[k][3], qf[k][half + 2]);
+                                for (int h = 0; h < 2; ++h)
+                                    qf[n][i][h] = pack_f16(__uint_as_float(qf[n][i][h] << 16) * scale, __uint_as_float(qf[n][i][h] & 0xffff0000u) * scale);
+                            }
                         }
                     }
-                    (half ? rs1 : rs0) = back * (a.softmax_scale * kLog2e);
+                    back *= a.softmax_scale * kLog2e;
+                    rs[n][0] = __shfl_sync(0xffffffffu, back, 8 * c);       // of row 2c
+                    rs[n][1] = __shfl_sync(0xffffffffu, back, 8 * c + 4);   // of row 2c + 1
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        ref[n][e] = -INFINITY;
+                        l[n][e] = 0.f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < DM; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
                 }
             }
-            const bool ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars[ring]), phase, give_up) ? 1 : 0) != 0;
-            if (!ok) break;
-            const uint32_t stage = ring0 + static_cast<uint32_t>(ring) * p.stage_bytes;
-            for (int ts = 0; ts < p.ts; ++ts) {
-                const int tile = ts * p.tw + tok;
-                const float4 mt = meta[ring * p.items + tile * p.hw + hl];
-                const int valid = static_cast<int>(mt.z);
-                if (valid == 0) continue;
-                const uint32_t kt = stage + static_cast<uint32_t>(tile) * NH * box_bytes + static_cast<uint32_t>(hl) * HEAD_TILE;
-                const uint32_t vt = kt + v_off;
-                // ---- S = Q Kc^T: tokens 0-7 and 8-15 ----
-                float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+            const int valid = __shfl_sync(0xffffffffu, cur.at, k) & 31;
+            const float ks = __shfl_sync(0xffffffffu, cur.ks, k), vs = __shfl_sync(0xffffffffu, cur.vs, k);
+            if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8u * slot, phase, give_up) ? 1 : 0)) break;
+            if (valid > 0) {
+                const uint32_t kt = ring0 + slot * STAGE;
+                // ---- S^T = Kc Q^T: 16 tokens by 8 query rows ----
+                float s[NT][4];
 #pragma unroll
-                for (int k = 0; k < CH; k += 4) {
-                    const int cc = (k % (RB / 16)) + (lane >> 3);
-                    const uint32_t at = kt + (k * 16 / RB) * box_bytes + krow * RB + ((cc ^ ksw) << 4);
+                for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+                for (int i = 0; i < CH; i += 4) {
+                    const int cc = (i % (RB / 16)) + (lane >> 3);
+                    const uint32_t at = kt + (i * 16 / RB) * BOX + krow * RB + ((cc ^ ksw) << 4);
                     uint32_t b[4], d[4];
-                    ldmatrix4(at, b);
-                    ldmatrix4(at + 8 * RB, d);
+                    ldmatrix4(at, b);            // tokens 0-7
+                    ldmatrix4(at + 8 * RB, d);   // tokens 8-15
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t lo, hi;
-                        codes_to_f16<E4M3>(b[i], lo, hi);
-                        mma_f16(s0, qf[k + i], lo, hi);
-                        if constexpr (SPLIT) mma_f16(s0, ql[k + i], lo, hi);
-                        codes_to_f16<E4M3>(d[i], lo, hi);
-                        mma_f16(s1, qf[k + i], lo, hi);
-                        if constexpr (SPLIT) mma_f16(s1, ql[k + i], lo, hi);
+                    for (int m = 0; m < 4; ++m) {
+                        uint32_t f[4];
+                        codes_to_f16<E4M3>(b[m], f[0], f[2]);
+                        codes_to_f16<E4M3>(d[m], f[1], f[3]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma_f16(s[n], f, qf[n][i + m][0], qf[n][i + m][1]);
+                            if constexpr (SPLIT) mma_f16(s[n], f, ql[n][i + m][0], ql[n][i + m][1]);
+                        }
                     }
                 }
                 // ---- weights against the tile's own maximum ----
-                // s0[0], s0[1]: row r0, tokens 2c, 2c + 1; s0[2], s0[3]: row r1; s1: the tokens eight further
-                float f0 = mt.x * rs0, f1 = mt.x * rs1;
-                const int pos = step * p.tt + tile * kTile;
+                // s[0], s[1]: token g, rows 2c, 2c + 1; s[2], s[3]: token g + 8
+                const int pos = (t - pre[req]) * kTile;
                 const bool whole = valid == kTile && pos + kTile <= lim_min;
-                if (!whole) {
-                    const int n0 = min(valid, lim0 - pos), n1 = min(valid, lim1 - pos);
+                uint32_t pb[NT][2], pl[NT][2];
+                float gain[NT][2];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        s0[i] = 2 * c + i < n0 ? s0[i] * f0 : -INFINITY;
-                        s1[i] = 2 * c + i + 8 < n0 ? s1[i] * f0 : -INFINITY;
-                        s0[i + 2] = 2 * c + i < n1 ? s0[i + 2] * f1 : -INFINITY;
-                        s1[i + 2] = 2 * c + i + 8 < n1 ? s1[i + 2] * f1 : -INFINITY;
+                for (int n = 0; n < NT; ++n) {
+                    float f0 = ks * rs[n][0], f1 = ks * rs[n][1];
+                    if (!whole) {
+                        const int r = rbase + 8 * n + 2 * c;
+                        const int n0 = min(valid, lim_min + r / group - pos), n1 = min(valid, lim_min + (r + 1) / group - pos);
+                        s[n][0] = g < n0 ? s[n][0] * f0 : -INFINITY;
+                        s[n][1] = g < n1 ? s[n][1] * f1 : -INFINITY;
+                        s[n][2] = g + 8 < n0 ? s[n][2] * f0 : -INFINITY;
+                        s[n][3] = g + 8 < n1 ? s[n][3] * f1 : -INFINITY;
+                        f0 = f1 = 1.f;
                     }
-                    f0 = f1 = 1.f;
-                }
-                float m0 = fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s1[0], s1[1]));
-                float m1 = fmaxf(fmaxf(s0[2], s0[3]), fmaxf(s1[2], s1[3]));
-                m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 1));
-                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
-                m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 2));
-                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
-                m0 = fmaxf(fmaf(m0, f0, -15.f), -1e30f);   // a row that sees nothing of the tile: every weight 2^-inf
-                m1 = fmaxf(fmaf(m1, f1, -15.f), -1e30f);
-                float p0[4], p1[4];
+                    float m0 = fmaxf(s[n][0], s[n][2]), m1 = fmaxf(s[n][1], s[n][3]);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    p0[i] = ex2_fast(fmaf(s0[i], f0, -m0));
-                    p1[i] = ex2_fast(fmaf(s1[i], f0, -m0));
-                    p0[i + 2] = ex2_fast(fmaf(s0[i + 2], f1, -m1));
-                    p1[i + 2] = ex2_fast(fmaf(s1[i + 2], f1, -m1));
-                }
-                if (__any_sync(0xffffffffu, m0 > ref0 + 40.f || m1 > ref1 + 40.f)) {
-                    const float n0 = fmaxf(ref0, m0), n1 = fmaxf(ref1, m1);
-                    const float a0 = ex2_fast(ref0 - n0), a1 = ex2_fast(ref1 - n1);
-                    ref0 = n0;
-                    ref1 = n1;
-                    l0 *= a0;
-                    l1 *= a1;
+                    for (int x = 4; x < 32; x *= 2) {
+                        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, x));
+                        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, x));
+                    }
+                    m0 = fmaxf(fmaf(m0, f0, -15.f), -1e30f);   // a row that sees nothing of the tile: every weight 2^-inf
+                    m1 = fmaxf(fmaf(m1, f1, -15.f), -1e30f);
+                    const float p0 = ex2_fast(fmaf(s[n][0], f0, -m0)), p1 = ex2_fast(fmaf(s[n][1], f1, -m1));
+                    const float p2 = ex2_fast(fmaf(s[n][2], f0, -m0)), p3 = ex2_fast(fmaf(s[n][3], f1, -m1));
+                    if (__any_sync(0xffffffffu, m0 > ref[n][0] + 40.f || m1 > ref[n][1] + 40.f)) {
+                        const float u0 = fmaxf(ref[n][0], m0), u1 = fmaxf(ref[n][1], m1);
+                        const float a0 = ex2_fast(ref[n][0] - u0), a1 = ex2_fast(ref[n][1] - u1);
+                        ref[n][0] = u0;
+                        ref[n][1] = u1;
+                        l[n][0] *= a0;
+                        l[n][1] *= a1;
 #pragma unroll
-                    for (int j = 0; j < DN; ++j) {
-                        o[j][0] *= a0;
-                        o[j][1] *= a0;
-                        o[j][2] *= a1;
-                        o[j][3] *= a1;
+                        for (int j = 0; j < DM; ++j) {
+                            o[n][j][0] *= a0;
+                            o[n][j][1] *= a1;
+                            o[n][j][2] *= a0;
+                            o[n][j][3] *= a1;
+                        }
+                    }
+                    const float w0 = ex2_fast(m0 - ref[n][0]), w1 = ex2_fast(m1 - ref[n][1]);
+                    l[n][0] = fmaf(p0 + p2, w0, l[n][0]);   // of tokens g and g + 8: the lanes are added up at the end
+                    l[n][1] = fmaf(p1 + p3, w1, l[n][1]);
+                    gain[n][0] = w0 * vs;
+                    gain[n][1] = w1 * vs;
+                    // P^T as a B fragment: row g, tokens 2c, 2c + 1 and 2c + 8, 2c + 9
+                    const uint32_t h0 = pack_f16(p0, p1), h1 = pack_f16(p2, p3);
+                    pb[n][0] = transpose8(h0);
+                    pb[n][1] = transpose8(h1);
+                    if constexpr (SPLIT) {
+                        pl[n][0] = transpose8(pack_rest(p0, p1, h0));
+                        pl[n][1] = transpose8(pack_rest(p2, p3, h1));
                     }
                 }
-                const float w0 = ex2_fast(m0 - ref0), w1 = ex2_fast(m1 - ref1);
-                l0 = fmaf((p0[0] + p0[1]) + (p1[0] + p1[1]), w0, l0);
-                l1 = fmaf((p0[2] + p0[3]) + (p1[2] + p1[3]), w1, l1);
-                const float g0 = w0 * mt.y, g1 = w1 * mt.y;
-                uint32_t pa[4], pl[4];
-                pa[0] = pack_f16(p0[0], p0[1]);
-                pa[1] = pack_f16(p0[2], p0[3]);
-                pa[2] = pack_f16(p1[0], p1[1]);
-                pa[3] = pack_f16(p1[2], p1[3]);
-                if constexpr (SPLIT) {
-                    pl[0] = pack_rest(p0[0], p0[1], pa[0]);
-                    pl[1] = pack_rest(p0[2], p0[3], pa[1]);
-                    pl[2] = pack_rest(p1[0], p1[1], pa[2]);
-                    pl[3] = pack_rest(p1[2], p1[3], pa[3]);
-                }
-                // ---- O += (w vs) (P Vc) ----
+                // ---- O^T += (w vs) (Vc^T P^T) ----
                 // Codes of tokens that do not exist are whatever the block holds, NaN perhaps: their weight is 0, so are they.
                 uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
                 if (valid < kTile) {
@@ -571,7 +525,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
 #pragma unroll
                 for (int h = 0; h < NH; ++h) {
                     uint32_t v[4][VB / 4];   // tokens 2c, 2c + 1, 2c + 8, 2c + 9
-                    const uint32_t vb = vt + h * box_bytes + v_lane;
+                    const uint32_t vb = kt + h * BOX + v_lane;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t trow = (i & 1) * RB + (i >> 1) * 8 * RB;
@@ -585,129 +539,98 @@ __global__ void __launch_bounds__(kQThreads, 1)
                     }
 #pragma unroll
                     for (int w = 0; w < VB / 4; ++w) {
-                        uint32_t b0[4], b1[4];
-                        codes_to_f16<E4M3>(__byte_perm(v[0][w], v[1][w], 0x5140) & keep0, b0[0], b0[1]);
-                        codes_to_f16<E4M3>(__byte_perm(v[0][w], v[1][w], 0x7362) & keep0, b0[2], b0[3]);
-                        codes_to_f16<E4M3>(__byte_perm(v[2][w], v[3][w], 0x5140) & keep1, b1[0], b1[1]);
-                        codes_to_f16<E4M3>(__byte_perm(v[2][w], v[3][w], 0x7362) & keep1, b1[2], b1[3]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float (&oj)[4] = o[h * VB + w * 4 + i];
-                            float tmp[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_f16(tmp, pa, b0[i], b1[i]);
-                            if constexpr (SPLIT) mma_f16(tmp, pl, b0[i], b1[i]);
-                            oj[0] = fmaf(tmp[0], g0, oj[0]);
-                            oj[1] = fmaf(tmp[1], g0, oj[1]);
-                            oj[2] = fmaf(tmp[2], g1, oj[2]);
-                            oj[3] = fmaf(tmp[3], g1, oj[3]);
-                        }
-                    }
-                }
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&bars[p.nstages + ring]));
-            if (++ring == p.nstages) {
-                ring = 0;
-                phase ^= 1u;
-            }
-            if (!last) continue;
-
-            // ---- the request's part in this CTA is done ----
-            l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-            l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-            l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-            l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-            bool fine = true;
-            // The warps of the same head and rows but other token tiles: the upper half hands its state over, until one is left.
-            constexpr int STATE = 4 * DN + 4;
-            for (int half = p.tw >> 1; half > 0 && fine; half >>= 1) {
-                float* box = red + static_cast<size_t>(((tok & (half - 1)) * p.mt + mtile) * p.hw + hl) * (STATE * 32) + lane;
-                if (tok >= half && tok < 2 * half) {
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t sel = i == 0 ? 0x5140 : 0x7362;
+                            uint32_t f[4];
+                            codes_to_f16<E4M3>(__byte_perm(v[0][w], v[1][w], sel) & keep0, f[0], f[1]);
+                            codes_to_f16<E4M3>(__byte_perm(v[2][w], v[3][w], sel) & keep1, f[2], f[3]);
 #pragma unroll
-                    for (int j = 0; j < DN; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) box[(4 * j + e) * 32] = o[j][e];
-                    box[(4 * DN) * 32] = ref0;
-                    box[(4 * DN + 1) * 32] = ref1;
-                    box[(4 * DN + 2) * 32] = l0;
-                    box[(4 * DN + 3) * 32] = l1;
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&bars[2 * p.nstages]));
-                fine = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars[2 * p.nstages]), merge_phase, give_up) ? 1 : 0) != 0;
-                if (!fine) break;
-                if (tok < half) {
-                    const float u0 = box[(4 * DN) * 32], u1 = box[(4 * DN + 1) * 32];
-                    const float n0 = fmaxf(fmaxf(ref0, u0), -1e30f), n1 = fmaxf(fmaxf(ref1, u1), -1e30f);
-                    const float a0 = ex2_fast(ref0 - n0), a1 = ex2_fast(ref1 - n1), b0 = ex2_fast(u0 - n0), b1 = ex2_fast(u1 - n1);
-                    ref0 = n0;
-                    ref1 = n1;
-                    l0 = fmaf(l0, a0, box[(4 * DN + 2) * 32] * b0);
-                    l1 = fmaf(l1, a1, box[(4 * DN + 3) * 32] * b1);
-#pragma unroll
-                    for (int j = 0; j < DN; ++j) {
-                        o[j][0] = fmaf(o[j][0], a0, box[(4 * j) * 32] * b0);
-                        o[j][1] = fmaf(o[j][1], a0, box[(4 * j + 1) * 32] * b0);
-                        o[j][2] = fmaf(o[j][2], a1, box[(4 * j + 2) * 32] * b1);
-                        o[j][3] = fmaf(o[j][3], a1, box[(4 * j + 3) * 32] * b1);
-                    }
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&bars[2 * p.nstages + 1]));
-                fine = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars[2 * p.nstages + 1]), merge_phase, give_up) ? 1 : 0) != 0;
-                merge_phase ^= 1u;
-            }
-            if (!fine) break;
-            if (tok > 0) continue;
-            // A request that this CTA has seen from its first step to its last one is finished here.
-            const bool alone = part_first == 0 && step + 1 == pre[req + 1] - pre[req];
-            const int64_t part = (static_cast<int64_t>(cta) + req) * a.n * a.Hq;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int r = half ? r1 : r0;
-                if (r >= R) continue;
-                const int64_t row = half ? row1 : row0;
-                const float l = half ? l1 : l0;
-                if (alone) {
-                    const float inv = l == 0.f ? 0.f : 1.f / l;
-                    const int tq = half ? tq1 : tq0;
-                    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(req) * a.o_s0 + static_cast<int64_t>(tq) * a.o_s1 +
-                             static_cast<int64_t>(hkv * group + (r - tq * group)) * a.o_s2;
-                    const bool vec = aligned16(out);
-#pragma unroll
-                    for (int h = 0; h < NH; ++h)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int d = h * RB + (2 * c + e) * VB;
-                            if (d >= a.D) continue;
-                            constexpr int VN = Vec16<T>::N;
-#pragma unroll
-                            for (int j = 0; j < VB; j += VN) {
-                                float f[VN];
-#pragma unroll
-                                for (int i = 0; i < VN; ++i) f[i] = o[h * VB + j + i][2 * half + e] * inv;
-                                if (vec) {
-                                    *reinterpret_cast<uint4*>(out + d + j) = pack16<T>(f);
-                                } else {
-#pragma unroll
-                                    for (int i = 0; i < VN; ++i) out[d + j + i] = Cvt<T>::from_f(f[i]);
-                                }
+                            for (int n = 0; n < NT; ++n) {
+                                float (&oj)[4] = o[n][h * (VB / 2) + w * 2 + i];
+                                float tmp[4] = {0.f, 0.f, 0.f, 0.f};
+                                mma_f16(tmp, f, pb[n][0], pb[n][1]);
+                                if constexpr (SPLIT) mma_f16(tmp, f, pl[n][0], pl[n][1]);
+                                oj[0] = fmaf(tmp[0], gain[n][0], oj[0]);
+                                oj[1] = fmaf(tmp[1], gain[n][1], oj[1]);
+                                oj[2] = fmaf(tmp[2], gain[n][0], oj[2]);
+                                oj[3] = fmaf(tmp[3], gain[n][1], oj[3]);
                             }
                         }
-                } else {
-                    float* acc = ws_acc + (part + row) * a.D;
+                    }
+                }
+            }
+
+            __syncwarp();
+            // ---- refill: the slot just read, or, where other warps read it too, the one before it ----
+            if (p.mt > 1 && lane == 0) mbar_arrive(empty0 + 8u * slot);
+            if (mtile == 0) {
+                const int lag = p.mt > 1 ? 1 : 0;
+                const int u = t - lag + p.stages;   // the tile to fetch
+                if (t - lag >= t0 && u < t1) {
+                    const int ku = u - base;
+                    const int from_block = ku < 32 ? cur.block : nxt.block, from_at = ku < 32 ? cur.at : nxt.at;
+                    const int block = __shfl_sync(0xffffffffu, from_block, ku & 31), at = __shfl_sync(0xffffffffu, from_at, ku & 31);
+                    const int to = slot >= lag ? slot - lag : p.stages - 1;
+                    if (lane == 0) {
+                        const uint32_t ph = to > slot ? phase ^ 1u : phase;   // the slot before slot 0 was read in the round before
+                        if (lag == 0 || mbar_wait(empty0 + 8u * to, ph, give_up)) fetch(to, block, at);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (++slot == p.stages) {
+                slot = 0;
+                phase ^= 1u;
+            }
+            if (t + 1 != req_end) continue;
+
+            // ---- the request's part in this range is done: written directly when it is all of it ----
+            const bool alone = part_first == 0 && t + 1 == pre[req + 1];
+            const int64_t part = (static_cast<int64_t>(range) + req) * a.n * a.Hq;
 #pragma unroll
-                    for (int h = 0; h < NH; ++h)
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int d = h * RB + (2 * c + e) * VB;
-                            if (d >= a.D) continue;
+                for (int x = 4; x < 32; x *= 2) {
+                    l[n][0] += __shfl_xor_sync(0xffffffffu, l[n][0], x);
+                    l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], x);
+                }
 #pragma unroll
-                            for (int j = 0; j < VB; j += 4)
-                                *reinterpret_cast<float4*>(acc + d + j) = make_float4(o[h * VB + j][2 * half + e], o[h * VB + j + 1][2 * half + e],
-                                                                                      o[h * VB + j + 2][2 * half + e], o[h * VB + j + 3][2 * half + e]);
+                for (int e = 0; e < 2; ++e) {
+                    const int r = rbase + 8 * n + 2 * c + e;
+                    if (r >= R) continue;
+                    const int tq = r / group, hq = hkv * group + (r - tq * group);
+                    const float inv = l[n][e] == 0.f ? 0.f : 1.f / l[n][e];
+                    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(req) * a.o_s0 + static_cast<int64_t>(tq) * a.o_s1 + static_cast<int64_t>(hq) * a.o_s2;
+                    const bool vec = aligned16(out);
+                    const int64_t row = part + static_cast<int64_t>(tq) * a.Hq + hq;
+#pragma unroll
+                    for (int h = 0; h < NH; ++h) {
+                        const int d = h * RB + g * VB;
+                        if (d >= a.D) continue;
+                        float f[VB];
+#pragma unroll
+                        for (int j = 0; j < VB; ++j) f[j] = o[n][h * (VB / 2) + j / 2][2 * (j & 1) + e];
+                        if (!alone) {
+#pragma unroll
+                            for (int j = 0; j < VB; j += 4) *reinterpret_cast<float4*>(ws_acc + row * a.D + d + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+                            continue;
                         }
-                    if (c == 0) *reinterpret_cast<float2*>(ws_ml + (part + row) * 2) = make_float2(half ? ref1 : ref0, l);
+                        constexpr int VN = Vec16<T>::N;
+#pragma unroll
+                        for (int j = 0; j < VB; j += VN) {
+                            float x[VN];
+#pragma unroll
+                            for (int i = 0; i < VN; ++i) x[i] = f[j + i] * inv;
+                            if (vec) {
+                                *reinterpret_cast<uint4*>(out + d + j) = pack16<T>(x);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < VN; ++i) out[d + j + i] = Cvt<T>::from_f(x[i]);
+                            }
+                        }
+                    }
+                    if (!alone && g == 0) *reinterpret_cast<float2*>(ws_ml + row * 2) = make_float2(ref[n][e], l[n][e]);
                 }
             }
         }
@@ -722,15 +645,20 @@ __global__ void __launch_bounds__(kQThreads, 1)
     }
 }
 
-// Merges the parts of a request that several CTAs had, and writes zeros for an empty one. One warp to a query row.
+// Merges the parts of a request that several ranges had, and writes zeros for an empty one. `wpr` warps share a query row: the
+// launch gives a row as many as it has parts for on average, as the parts of one long request are too many for one warp to
+// read one after the other (four requests of 30011 to 131072 tokens: 145 us with one warp to a row, 5 us with eight).
+constexpr int kMergeWarps = 8;
+
 template <typename T>
-__global__ void __launch_bounds__(128) quant_combine_kernel(const QuantAttnArgs a, int tt, int n_cta, const float* __restrict__ ws_acc,
-                                                            const float* __restrict__ ws_ml) {
-    __shared__ int s_part[4][2];
+__global__ void __launch_bounds__(32 * kMergeWarps) quant_combine_kernel(const QuantAttnArgs a, int n_range, int wpr, const float* __restrict__ ws_acc,
+                                                                         const float* __restrict__ ws_ml) {
+    __shared__ int s_part[kMergeWarps][2];
+    __shared__ float s_acc[kMergeWarps][32 * 8 + 1];
     const int i = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int before = 0, all = 0;
-    for (int r = threadIdx.x; r < a.B; r += blockDim.x) {
-        const int n = (quant_len(a, r) + tt - 1) / tt;
+    for (int r = threadIdx.x; r < a.B; r += 32 * kMergeWarps) {
+        const int n = (quant_len(a, r) + kTile - 1) / kTile;
         all += n;
         if (r < i) before += n;
     }
@@ -744,50 +672,87 @@ __global__ void __launch_bounds__(128) quant_combine_kernel(const QuantAttnArgs 
         s_part[warp][1] = all;
     }
     __syncthreads();
-    before = s_part[0][0] + s_part[1][0] + s_part[2][0] + s_part[3][0];
-    all = s_part[0][1] + s_part[1][1] + s_part[2][1] + s_part[3][1];
-    const int steps = (quant_len(a, i) + tt - 1) / tt;
-    const int used = used_ctas(all, n_cta);
-    // CTA c has the steps [all * c / used, all * (c + 1) / used): every one of the used CTAs has some.
-    int c_first = 0, c_last = -1;
-    if (steps > 0) {
-        auto cta_of = [&](int t) {
+    before = all = 0;
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; ++w) {
+        before += s_part[w][0];
+        all += s_part[w][1];
+    }
+    const int tiles = (quant_len(a, i) + kTile - 1) / kTile;
+    const int used = used_ranges(all, n_range);
+    // Range c has the tiles [all * c / used, all * (c + 1) / used): every one of the used ranges has some.
+    int c_first = 0, parts = 0;
+    if (tiles > 0) {
+        auto range_of = [&](int t) {
             const int64_t c = ((static_cast<int64_t>(t) + 1) * used - 1) / all;
             return static_cast<int>(c < used - 1 ? c : used - 1);
         };
-        c_first = cta_of(before);
-        c_last = cta_of(before + steps - 1);
-        if (c_first == c_last) return;   // written by that CTA
+        c_first = range_of(before);
+        parts = range_of(before + tiles - 1) - c_first + 1;
+        if (parts == 1) return;   // written by that range
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int row = blockIdx.y * 4 + warp;
-    if (row >= a.n * a.Hq) return;
-    constexpr int RG = 8;   // head_dim <= 256
-    float acc[RG];
-#pragma unroll
-    for (int r = 0; r < RG; ++r) acc[r] = 0.f;
+    const int row = blockIdx.y * (kMergeWarps / wpr) + warp / wpr, sub = warp % wpr;
+    const bool here = row < a.n * a.Hq;
     const int64_t rows = static_cast<int64_t>(a.n) * a.Hq;
-    float M = -INFINITY, L = 0.f;
-    for (int c = c_first; c <= c_last; ++c) M = fmaxf(M, ws_ml[((static_cast<int64_t>(c) + i) * rows + row) * 2]);
-    M = fmaxf(M, -1e30f);
-    for (int c = c_first; c <= c_last; ++c) {
-        const int64_t at = (static_cast<int64_t>(c) + i) * rows + row;
-        const float2 ml = *reinterpret_cast<const float2*>(ws_ml + at * 2);
-        const float w = exp2f(ml.x - M);
-        L = fmaf(ml.y, w, L);
+    const float* ml = ws_ml + ((static_cast<int64_t>(c_first) + i) * rows + row) * 2;
+    const float* acc = ws_acc + ((static_cast<int64_t>(c_first) + i) * rows + row) * a.D;
+    float v[8];   // d = 4 * lane .. + 3, and 128 further
 #pragma unroll
-        for (int r = 0; r < RG; ++r) {
-            const int d = lane + 32 * r;
-            if (d < a.D) acc[r] = fmaf(ws_acc[at * a.D + d], w, acc[r]);
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    float L = 0.f;
+    if (here) {
+        float M = -1e30f;
+        for (int c = lane; c < parts; c += 32) M = fmaxf(M, ml[c * rows * 2]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const bool d0 = 4 * lane < a.D, d1 = 4 * lane + 128 < a.D;
+        for (int c = sub; c < parts; c += 4 * wpr) {
+            float2 x[4];
+            float4 y[4], z[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t at = (c + u * wpr) * rows;
+                const bool in = c + u * wpr < parts;
+                x[u] = in ? *reinterpret_cast<const float2*>(ml + at * 2) : make_float2(-INFINITY, 0.f);
+                y[u] = in && d0 ? *reinterpret_cast<const float4*>(acc + at * a.D + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+                z[u] = in && d1 ? *reinterpret_cast<const float4*>(acc + at * a.D + 4 * lane + 128) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float w = exp2f(x[u].x - M);
+                L = fmaf(x[u].y, w, L);
+                v[0] = fmaf(y[u].x, w, v[0]);
+                v[1] = fmaf(y[u].y, w, v[1]);
+                v[2] = fmaf(y[u].z, w, v[2]);
+                v[3] = fmaf(y[u].w, w, v[3]);
+                v[4] = fmaf(z[u].x, w, v[4]);
+                v[5] = fmaf(z[u].y, w, v[5]);
+                v[6] = fmaf(z[u].z, w, v[6]);
+                v[7] = fmaf(z[u].w, w, v[7]);
+            }
         }
     }
+    if (wpr > 1) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s_acc[warp][e * 32 + lane] = v[e];
+        if (lane == 0) s_acc[warp][256] = L;
+        __syncthreads();
+        if (sub != 0) return;
+        for (int w = 1; w < wpr; ++w) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += s_acc[warp + w][e * 32 + lane];
+            L += s_acc[warp + w][256];
+        }
+    }
+    if (!here) return;
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const int t = row / a.Hq, h = row - t * a.Hq;
     T* out = static_cast<T*>(a.out) + static_cast<int64_t>(i) * a.o_s0 + static_cast<int64_t>(t) * a.o_s1 + static_cast<int64_t>(h) * a.o_s2;
 #pragma unroll
-    for (int r = 0; r < RG; ++r) {
-        const int d = lane + 32 * r;
-        if (d < a.D) out[d] = Cvt<T>::from_f(acc[r] * inv);
+    for (int e = 0; e < 8; ++e) {
+        const int d = 4 * lane + (e & 3) + (e >> 2) * 128;
+        if (d < a.D) out[d] = Cvt<T>::from_f(v[e] * inv);
     }
 }
 
@@ -809,7 +774,7 @@ EncodeFn encode_fn() {
     return fn;
 }
 
-// [head_dim, position, head, block] of one cache whatever its strides; a box is 16 positions of hw heads. Bytes of a row
+// [head_dim, position, head, block] of one cache whatever its strides; a box is 16 positions of a head. Bytes of a row
 // beyond head_dim arrive as zeros.
 bool encode_map(const QuantAttnArgs& a, const QuantPlan& p, int m, CUtensorMap* map) {
     EncodeFn fn = encode_fn();
@@ -818,7 +783,7 @@ bool encode_map(const QuantAttnArgs& a, const QuantPlan& p, int m, CUtensorMap* 
     auto stride = [](int64_t s, int64_t extent) { return static_cast<cuuint64_t>(extent > 1 ? s : 16); };
     const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.D), static_cast<cuuint64_t>(a.block_size), static_cast<cuuint64_t>(a.Hkv), static_cast<cuuint64_t>(a.blocks)};
     const cuuint64_t strides[3] = {stride(a.c_s1[m], a.block_size), stride(a.c_s2[m], a.Hkv), stride(a.c_s0[m], a.blocks)};
-    const cuuint32_t box[4] = {static_cast<cuuint32_t>(rb), kTile, static_cast<cuuint32_t>(p.hw), 1};
+    const cuuint32_t box[4] = {static_cast<cuuint32_t>(rb), kTile, 1, 1};
     const cuuint32_t ones[4] = {1, 1, 1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(a.cache[m]), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
               rb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
@@ -828,8 +793,7 @@ bool encode_map(const QuantAttnArgs& a, const QuantPlan& p, int m, CUtensorMap* 
 // Whether the split kernel takes these arguments, and how it cuts them.
 bool make_quant_plan(const QuantAttnArgs& a, int sm_count, int max_smem, QuantPlan& p) {
     if (a.force_plain || a.D % 16 != 0 || a.block_size % kTile != 0 || a.blocks <= 0 || a.cols <= 0) return false;
-    // head_dim 256 in fp32 would need 128 registers of query fragments beside 128 of accumulators
-    if (a.D > 256 || (a.dt == Dt::F32 && a.D > 128)) return false;
+    if (a.D > 256) return false;
     if (a.B > kQMaxB || static_cast<int64_t>(a.B) * a.cols * a.block_size / kTile >= (1ll << 30) || a.blocks >= (1ll << 31)) return false;
     for (int m = 0; m < 2; ++m) {
         auto ok = [](int64_t s, int64_t extent) { return extent <= 1 || (s > 0 && s % 16 == 0 && s < (1ll << 40)); };
@@ -840,76 +804,86 @@ bool make_quant_plan(const QuantAttnArgs& a, int sm_count, int max_smem, QuantPl
     p = QuantPlan{};
     p.hd = a.D <= 64 ? 64 : a.D <= 128 ? 128 : 256;
     const int R = a.n * (a.Hq / a.Hkv);
-    p.mt = 1;
-    while (p.mt < kQWarps && p.mt * 16 < R) p.mt *= 2;
-    p.n_z = (R + p.mt * 16 - 1) / (p.mt * 16);
-    p.hw = 1;
-    for (int h = 2; h <= kQWarps / p.mt; ++h)
-        if (a.Hkv % h == 0) p.hw = h;
+    const bool f32 = a.dt == Dt::F32;
+    p.nt = R > 8 && p.hd <= 128 && !f32 ? 2 : 1;
+    const int warps = split_warps(f32, p.hd, p.nt);
+    p.mt = std::min((R + 8 * p.nt - 1) / (8 * p.nt), warps);
+    p.n_z = (R + p.mt * 8 * p.nt - 1) / (p.mt * 8 * p.nt);
+    // Heads of a CTA: the divisor of Hkv that keeps most warps busy, the largest of those.
+    int busy = 0;
+    for (int h = 1; h <= warps / p.mt; ++h) {
+        const int b = h * (warps / p.mt / h);
+        if (a.Hkv % h == 0 && h <= 8 && b >= busy) {
+            busy = b;
+            p.hw = h;
+        }
+    }
     p.n_hg = a.Hkv / p.hw;
-    p.tw = 1;
-    while (p.hw * p.mt * p.tw * 2 <= kQWarps) p.tw *= 2;
-    // A step of about 32 KB: enough bytes to pay for its hand-over, and still six of them in flight.
-    const int pair = 2 * kTile * p.hd;   // K and V of a tile
-    p.ts = 1;
-    while (p.hw * p.tw * p.ts * 2 * pair <= 32768 && p.hw * p.tw * p.ts * 2 <= 16) p.ts *= 2;
-    p.tt = kTile * p.tw * p.ts;
-    p.items = p.hw * p.tw * p.ts;
-    p.stage_bytes = p.items * pair;
-    const int state = (4 * (p.hd / 8) + 4) * 32 * 4;
-    const int red_bytes = p.tw > 1 ? p.tw / 2 * p.mt * p.hw * state : 0;
-    const int fixed = 1024 + kQMaxStages * p.items * 16 + (2 * kQMaxStages + 2) * 8 + (2 * a.B + 1) * 4 + red_bytes + 64;
-    p.nstages = std::min((max_smem - fixed) / p.stage_bytes, kQMaxStages);
-    if (p.nstages < 2) return false;
-    int off = p.nstages * p.stage_bytes;
+    p.tw = warps / p.mt / p.hw;
+    const int teams = p.hw * p.tw, stage = 2 * kTile * p.hd;
+    const int fixed = 1024 + teams * 2 * kQMaxStages * 8 + (2 * a.B + 1) * 4 + 64;
+    p.stages = std::min((max_smem - fixed) / (teams * stage), kQMaxStages);
+    if (p.stages < 2) return false;
+    int off = teams * p.stages * stage;
     auto take = [&](int bytes) {
         const int at = off;
         off += (bytes + 15) / 16 * 16;
         return at;
     };
-    p.off_meta = take(p.nstages * p.items * 16);
-    p.off_bars = take((2 * p.nstages + 2) * 8);
-    p.off_red = take(red_bytes);
+    p.off_bars = take(teams * 2 * p.stages * 8);
     p.off_pre = take((a.B + 1) * 4);
     p.off_len = take(a.B * 4);
     p.off_flag = take(4);
     p.smem_bytes = off + 1024;
     if (p.smem_bytes > max_smem) return false;
-    const int64_t most = static_cast<int64_t>(a.B) * ((static_cast<int64_t>(a.cols) * a.block_size + p.tt - 1) / p.tt);
-    p.n_cta = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count / (p.n_hg * p.n_z), (most + kStepsPerCta - 1) / kStepsPerCta)));
+    const int64_t most = static_cast<int64_t>(a.B) * ((static_cast<int64_t>(a.cols) * a.block_size + kTile - 1) / kTile);
+    const int64_t ranges = std::max<int64_t>(1, (most + kTilesPerRange - 1) / kTilesPerRange);
+    p.n_cta = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count / (p.n_hg * p.n_z), (ranges + p.tw - 1) / p.tw)));
+    p.n_range = p.n_cta * p.tw;
     const int64_t el = a.dt == Dt::F32 ? 4 : 2;
     p.qvec = reinterpret_cast<uintptr_t>(a.q) % (4 * el) == 0 && a.q_s0 % 4 == 0 && a.q_s1 % 4 == 0 && a.q_s2 % 4 == 0;
     return true;
 }
 
-int64_t part_rows(const QuantAttnArgs& a, const QuantPlan& p) { return (static_cast<int64_t>(p.n_cta) + a.B) * a.n * a.Hq; }
+int64_t part_rows(const QuantAttnArgs& a, const QuantPlan& p) { return (static_cast<int64_t>(p.n_range) + a.B) * a.n * a.Hq; }
 
-template <typename T, bool E4M3, int HD>
+template <typename T, bool E4M3, int HD, int NT>
 void launch_split(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap& mk, const CUtensorMap& mv, float* acc, float* ml, cudaStream_t st) {
-    auto kern = quant_split_kernel<T, E4M3, HD>;
+    auto kern = quant_split_kernel<T, E4M3, HD, NT>;
+    constexpr int threads = 32 * split_warps(std::is_same<T, float>::value, HD, NT);
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem_bytes);
-    kern<<<dim3(p.n_cta, p.n_hg, p.n_z), kQThreads, p.smem_bytes, st>>>(a, p, mk, mv, acc, ml);
+    kern<<<dim3(p.n_cta, p.n_hg, p.n_z), threads, p.smem_bytes, st>>>(a, p, mk, mv, acc, ml);
+    int wpr = 1;
+    while (wpr < kMergeWarps && wpr * 4 * a.B < p.n_range) wpr *= 2;   // parts of a request on average, four to a warp
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.B, (a.n * a.Hq + 3) / 4, 1);
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3(a.B, (a.n * a.Hq + kMergeWarps / wpr - 1) / (kMergeWarps / wpr), 1);
+    cfg.blockDim = dim3(32 * kMergeWarps);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, quant_combine_kernel<T>, a, p.tt, p.n_cta, static_cast<const float*>(acc), static_cast<const float*>(ml));
+    cudaLaunchKernelEx(&cfg, quant_combine_kernel<T>, a, p.n_range, wpr, static_cast<const float*>(acc), static_cast<const float*>(ml));
 }
 
 template <typename T>
 void launch_split_t(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap& mk, const CUtensorMap& mv, float* acc, float* ml, cudaStream_t st) {
-    if (p.hd == 64) {
-        a.e4m3 ? launch_split<T, true, 64>(a, p, mk, mv, acc, ml, st) : launch_split<T, false, 64>(a, p, mk, mv, acc, ml, st);
-    } else if (p.hd == 128) {
-        a.e4m3 ? launch_split<T, true, 128>(a, p, mk, mv, acc, ml, st) : launch_split<T, false, 128>(a, p, mk, mv, acc, ml, st);
-    } else if constexpr (!std::is_same<T, float>::value) {
-        a.e4m3 ? launch_split<T, true, 256>(a, p, mk, mv, acc, ml, st) : launch_split<T, false, 256>(a, p, mk, mv, acc, ml, st);
-    }
+    auto go = [&](auto e4m3, auto hd) {
+        if constexpr (!std::is_same<T, float>::value && hd.value <= 128) {
+            if (p.nt == 2) return launch_split<T, e4m3.value, hd.value, 2>(a, p, mk, mv, acc, ml, st);
+        }
+        launch_split<T, e4m3.value, hd.value, 1>(a, p, mk, mv, acc, ml, st);
+    };
+    auto widths = [&](auto e4m3) {
+        if (p.hd == 64)
+            go(e4m3, std::integral_constant<int, 64>{});
+        else if (p.hd == 128)
+            go(e4m3, std::integral_constant<int, 128>{});
+        else
+            go(e4m3, std::integral_constant<int, 256>{});
+    };
+    a.e4m3 ? widths(std::true_type{}) : widths(std::false_type{});
 }
 
 }  // namespace
