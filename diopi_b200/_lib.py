@@ -81,6 +81,10 @@ def load() -> _Libs:
     rt.b200rt_tensor_create.argtypes = [c_void_p, c_int, POINTER(c_int64), POINTER(c_int64), c_int, c_int]
     rt.b200rt_tensor_destroy.restype = None
     rt.b200rt_tensor_destroy.argtypes = [c_void_p]
+    rt.b200rt_batch_create.restype = c_void_p
+    rt.b200rt_batch_create.argtypes = [c_void_p, c_int, c_void_p]
+    rt.b200rt_batch_destroy.restype = None
+    rt.b200rt_batch_destroy.argtypes = [c_void_p]
     rt.b200rt_context_create.restype = c_void_p
     rt.b200rt_context_create.argtypes = [c_void_p, c_int]
     rt.b200rt_context_set_stream.restype = None

@@ -24,6 +24,7 @@
 // quant_plain_kernel: any width, strides and block size; one CTA to a query row, a warp to every fourth token.
 #include <cuda.h>
 
+#include <atomic>
 #include <mutex>
 #include <type_traits>
 
@@ -848,10 +849,17 @@ bool make_quant_plan(const QuantAttnArgs& a, int sm_count, int max_smem, QuantPl
 int64_t part_rows(const QuantAttnArgs& a, const QuantPlan& p) { return (static_cast<int64_t>(p.n_range) + a.B) * a.n * a.Hq; }
 
 template <typename T, bool E4M3, int HD, int NT>
-void launch_split(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap& mk, const CUtensorMap& mv, float* acc, float* ml, cudaStream_t st) {
+void launch_split(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap& mk, const CUtensorMap& mv, float* acc, float* ml, int max_smem, cudaStream_t st) {
     auto kern = quant_split_kernel<T, E4M3, HD, NT>;
     constexpr int threads = 32 * split_warps(std::is_same<T, float>::value, HD, NT);
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem_bytes);
+    // once per kernel and device: the call is not free, and the limit may as well be the device's
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !(done.load(std::memory_order_acquire) >> dev & 1)) {
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, max_smem);
+        if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+    }
     kern<<<dim3(p.n_cta, p.n_hg, p.n_z), threads, p.smem_bytes, st>>>(a, p, mk, mv, acc, ml);
     int wpr = 1;
     while (wpr < kMergeWarps && wpr * 4 * a.B < p.n_range) wpr *= 2;   // parts of a request on average, four to a warp
@@ -868,12 +876,12 @@ void launch_split(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap&
 }
 
 template <typename T>
-void launch_split_t(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap& mk, const CUtensorMap& mv, float* acc, float* ml, cudaStream_t st) {
+void launch_split_t(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap& mk, const CUtensorMap& mv, float* acc, float* ml, int max_smem, cudaStream_t st) {
     auto go = [&](auto e4m3, auto hd) {
         if constexpr (!std::is_same<T, float>::value && hd.value <= 128) {
-            if (p.nt == 2) return launch_split<T, e4m3.value, hd.value, 2>(a, p, mk, mv, acc, ml, st);
+            if (p.nt == 2) return launch_split<T, e4m3.value, hd.value, 2>(a, p, mk, mv, acc, ml, max_smem, st);
         }
-        launch_split<T, e4m3.value, hd.value, 1>(a, p, mk, mv, acc, ml, st);
+        launch_split<T, e4m3.value, hd.value, 1>(a, p, mk, mv, acc, ml, max_smem, st);
     };
     auto widths = [&](auto e4m3) {
         if (p.hd == 64)
@@ -902,11 +910,11 @@ const char* launch_quantized_attention(const QuantAttnArgs& a, void* ws, int sm_
         float* acc = reinterpret_cast<float*>(base);
         float* ml = acc + part_rows(a, p) * a.D;
         if (a.dt == Dt::F16)
-            launch_split_t<__half>(a, p, mk, mv, acc, ml, st);
+            launch_split_t<__half>(a, p, mk, mv, acc, ml, max_smem, st);
         else if (a.dt == Dt::BF16)
-            launch_split_t<__nv_bfloat16>(a, p, mk, mv, acc, ml, st);
+            launch_split_t<__nv_bfloat16>(a, p, mk, mv, acc, ml, max_smem, st);
         else
-            launch_split_t<float>(a, p, mk, mv, acc, ml, st);
+            launch_split_t<float>(a, p, mk, mv, acc, ml, max_smem, st);
         return "split";
     }
     const dim3 grid(a.B, a.n * a.Hq);

@@ -10,7 +10,7 @@
 //
 // Bytes: T * H * D * (e + 1) for each of K and V. One pass: the rows of a block stay in registers between the maximum and
 // the codes. A unit is one (request, block, head) of one matrix; 16 rows of it belong to a warp, with 16 elements of a row to
-// a lane (one 16-byte store of codes), and ceil(block_size / 16) warps (up to 8) share a unit through shared memory. Blocks
+// a lane, and ceil(block_size / 16) warps (up to 8) share a unit through shared memory. Blocks
 // of more than 128 rows are read twice (the second time from L1/L2).
 #include <cuda_fp8.h>
 
@@ -51,8 +51,9 @@ __device__ __forceinline__ float pow2f(int k) { return k < -149 ? 0.f : exp2f(st
 
 // One value, any input: the definition itself in double (a quotient of two fp32 values is never close enough to a tie of
 // an 8-bit format, without being one, for the double rounding to matter).
-__device__ __noinline__ uint32_t encode_slow(float x, float s, bool e4m3) {
-    if (e4m3) {
+template <bool E4M3>
+__device__ __noinline__ uint32_t encode_slow(float x, float s) {
+    if (E4M3) {
         if (isnan(x)) return 0x7fu;
         if (s == 0.f) return 0u;
         const float y = static_cast<float>(static_cast<double>(x) / static_cast<double>(s));   // s is a power of two
@@ -73,8 +74,9 @@ __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
 // Four codes. `inv` = 1 / s (exact for the powers of two of e4m3). int8: adding 1.5 * 2^23 rounds x * inv to an integer,
 // which sits in the low byte; x * inv carries the error of inv, so where the remainder x - q * s (exact in one fma: |q| <=
 // 127) is half a step or more the nearest code may be another one and `off` asks for the slow path.
-__device__ __forceinline__ uint32_t encode4(const float* x, float s, float inv, bool e4m3, float& off) {
-    if (e4m3) return e4m3_pair(x[0] * inv, x[1] * inv) | (e4m3_pair(x[2] * inv, x[3] * inv) << 16);
+template <bool E4M3>
+__device__ __forceinline__ uint32_t encode4(const float* x, float s, float inv, float& off) {
+    if (E4M3) return e4m3_pair(x[0] * inv, x[1] * inv) | (e4m3_pair(x[2] * inv, x[3] * inv) << 16);
     constexpr float kMagic = 12582912.f;
     uint32_t b[4];
 #pragma unroll
@@ -161,38 +163,62 @@ __device__ __forceinline__ CopyUnit find_unit(const QuantCopyArgs& a, int u) {
     return un;
 }
 
-// The 16 elements [16 * cl, 16 * cl + 16) of a row in fp32.
-template <typename T>
+// A lane's 16 elements of a row: vectors of 16 bytes, LPR lanes apart, so that a load covers whole lines.
+template <typename T, int LPR>
 struct Row16 {
-    static constexpr int N = 16 / Vec16<T>::N;   // 16-byte vectors
+    static constexpr int N = 16 / Vec16<T>::N;   // vectors
+    static constexpr int E = Vec16<T>::N;        // elements of one
     uint4 v[N];
-    __device__ __forceinline__ void load(const T* p) {
+    static __device__ __forceinline__ int col(int i, int cl) { return (i * LPR + cl) * E; }   // first element of vector i
+    __device__ __forceinline__ void load(const T* row, int cl, int D, bool in) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        for (int i = 0; i < N; ++i) v[i] = in && col(i, cl) < D ? __ldg(reinterpret_cast<const uint4*>(row + col(i, cl))) : make_uint4(0, 0, 0, 0);
     }
-    __device__ __forceinline__ void clear() {
+    // The bits of the largest magnitude as fp32: above those of infinity if there is a NaN, equal if there is an infinity.
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0;
+        if constexpr (sizeof(T) == 2) {
+            // magnitudes of a 16-bit float type are ordered as integers
+            uint32_t u = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < N; ++i) u = __vmaxu2(__vmaxu2(u, __vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu)), __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
+            const uint32_t w = max(u & 0xffffu, u >> 16);
+            const unsigned short h = static_cast<unsigned short>(w);
+            m = __float_as_uint(Cvt<T>::to_f(*reinterpret_cast<const T*>(&h))) & 0x7fffffffu;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                m = max(max(m, max(v[i].x & 0x7fffffffu, v[i].y & 0x7fffffffu)), max(v[i].z & 0x7fffffffu, v[i].w & 0x7fffffffu));
+        }
+        return m;
     }
-    __device__ __forceinline__ void unpack(float (&f)[16]) const {
+    __device__ __forceinline__ float finite_top() const {
+        float m = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            float g[Vec16<T>::N];
-            unpack16<T>(v[i], g);
+            float f[E];
+            unpack16<T>(v[i], f);
 #pragma unroll
-            for (int j = 0; j < Vec16<T>::N; ++j) f[i * Vec16<T>::N + j] = g[j];
+            for (int j = 0; j < E; ++j) m = fmaxf(m, isfinite(f[j]) ? fabsf(f[j]) : 0.f);
         }
+        return m;
     }
 };
 
-// Lanes of a row LPR (power of two, 16 elements each; lanes beyond D / 16 idle), W warps of 16 rows to a unit.
-template <typename T, int LPR, int W, bool REREAD>
-__global__ void __launch_bounds__(kCopyThreads) quantized_copy_kernel(const QuantCopyArgs a) {
+constexpr uint32_t kInfBits = 0x7f800000u;
+
+// CTAs of an SM that the registers are to leave room for: the rows of a warp's 16 are held between the two passes.
+template <typename T>
+constexpr int copy_ctas(int lpr) { return sizeof(T) * lpr <= 16 ? 4 : sizeof(T) * lpr <= 32 ? 2 : 1; }
+
+// Lanes of a row LPR (16 elements each; where the row is shorter some vectors are left out), W warps of 16 rows to a unit.
+template <typename T, bool E4M3, int LPR, int W, bool REREAD>
+__global__ void __launch_bounds__(kCopyThreads, copy_ctas<T>(LPR)) quantized_copy_kernel(const QuantCopyArgs a) {
+    using Row = Row16<T, LPR>;
     constexpr int RPP = 32 / LPR;              // rows of a warp's pass
     constexpr int PASSES = kWarpRows / RPP;
     constexpr int UPC = kCopyWarps / W;        // heads of a CTA
-    __shared__ float s_amax[kCopyWarps];
-    __shared__ int s_odd[kCopyWarps];
+    __shared__ uint32_t s_top[2][kCopyWarps];
     const int m = blockIdx.z;                  // 0: K, 1: V
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const CopyUnit un = find_unit(a, blockIdx.x);
@@ -200,85 +226,69 @@ __global__ void __launch_bounds__(kCopyThreads) quantized_copy_kernel(const Quan
     const int h = blockIdx.y * UPC + warp / W, wu = warp % W;
     const bool here = h < a.H;
     const int rl = lane / LPR, cl = lane % LPR;
-    const bool col = here && cl * 16 < a.D;
-    const T* src = static_cast<const T*>(a.src[m]) + static_cast<int64_t>(h) * a.src_s1[m] + cl * 16;
-    uint8_t* dst = static_cast<uint8_t*>(a.cache[m]) + un.block * a.c_s0[m] + static_cast<int64_t>(h) * a.c_s2[m] + cl * 16;
+    const T* src = static_cast<const T*>(a.src[m]) + static_cast<int64_t>(h) * a.src_s1[m];
+    uint8_t* dst = static_cast<uint8_t*>(a.cache[m]) + un.block * a.c_s0[m] + static_cast<int64_t>(h) * a.c_s2[m];
     float* scale = a.scale[m] + un.block * a.s_s0[m] + static_cast<int64_t>(h) * a.s_s1[m];
 
     // Row of pass i of chunk q in the block. Only the rows of the call are loaded.
     const int chunks = REREAD ? (un.p1 + W * kWarpRows - 1) / (W * kWarpRows) : 1;
     auto row_of = [&](int q, int i) { return (q * W + wu) * kWarpRows + i * RPP + rl; };
-    Row16<T> r[PASSES];
+    Row r[PASSES];
     auto load_rows = [&](int q) {
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
             const int p = row_of(q, i);
-            if (col && p >= un.p0 && p < un.p1)
-                r[i].load(src + (un.row0 + (p - un.p0)) * a.src_s0[m]);
-            else
-                r[i].clear();
+            const bool in = here && p >= un.p0 && p < un.p1;
+            r[i].load(src + (un.row0 + (in ? p - un.p0 : 0)) * a.src_s0[m], cl, a.D, in);
         }
     };
     const float old = here && un.p0 > 0 ? *scale : 0.f;   // read by every lane before the barrier below, written after it
 
-    float amax = 0.f;
-    int odd = 0;   // a NaN or an infinity among the rows
+    uint32_t top = 0;
     for (int q = 0; q < chunks; ++q) {
         load_rows(q);
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            float f[16];
-            r[i].unpack(f);
-            float mx = 0.f, chk = 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                mx = fmaxf(mx, fabsf(f[e]));
-                chk = fmaf(f[e], 0.f, chk);   // NaN for a NaN or an infinity
-            }
-            if (chk != 0.f) {
-                odd = 1;
-                mx = 0.f;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, isfinite(f[e]) ? fabsf(f[e]) : 0.f);
-            }
-            amax = fmaxf(amax, mx);
-        }
+        for (int i = 0; i < PASSES; ++i) top = max(top, r[i].top());
     }
+    auto over_unit = [&](uint32_t x, int buf) {   // the largest of a unit
+        x = __reduce_max_sync(0xffffffffu, x);
+        if constexpr (W > 1) {
+            if (lane == 0) s_top[buf][warp] = x;
+            __syncthreads();
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    odd = __any_sync(0xffffffffu, odd);
-    if constexpr (W > 1) {
-        if (lane == 0) {
-            s_amax[warp] = amax;
-            s_odd[warp] = odd;
+            for (int w = 0; w < W; ++w) x = max(x, s_top[buf][warp / W * W + w]);
         }
-        __syncthreads();
+        return x;
+    };
+    top = over_unit(top, 0);
+    const bool odd = top >= kInfBits;   // a NaN or an infinity in the unit: it does not count
+    if (W > 1 ? __syncthreads_or(odd) != 0 : odd) {
+        uint32_t f = 0;
+        for (int q = 0; q < chunks; ++q) {
+            if (REREAD) load_rows(q);
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            amax = fmaxf(amax, s_amax[warp / W * W + w]);
-            odd |= s_odd[warp / W * W + w];
+            for (int i = 0; i < PASSES; ++i) f = max(f, __float_as_uint(r[i].finite_top()));
         }
-    } else {
-        __syncwarp();
+        top = over_unit(f, 1);
     }
     if (!here) return;
 
-    float s = fresh_scale(amax, a.e4m3);
+    float s = fresh_scale(__uint_as_float(top), E4M3);
     if (un.p0 > 0 && old > 0.f) {
         const int steps = growth_steps(old, s);
         s = steps > 0 ? static_cast<float>(scalbn(static_cast<double>(old), steps)) : old;
         if (steps > 0) {   // what earlier calls left in this block, in the grown scale
             const float f = pow2f(-steps);
             for (int p = wu * kWarpRows + rl; p < un.p0; p += (p % kWarpRows + RPP < kWarpRows) ? RPP : (W - 1) * kWarpRows + RPP) {
-                if (!col) continue;
-                uint4* at = reinterpret_cast<uint4*>(dst + static_cast<int64_t>(p) * a.c_s1[m]);
+                if (cl * 16 >= a.D) continue;
+                uint4* at = reinterpret_cast<uint4*>(dst + static_cast<int64_t>(p) * a.c_s1[m] + cl * 16);
                 uint4 v = *at;
                 uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     uint32_t o = 0;
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) o |= shrink_code((w[e] >> (8 * b)) & 0xffu, f, a.e4m3) << (8 * b);
+                    for (int b = 0; b < 4; ++b) o |= shrink_code((w[e] >> (8 * b)) & 0xffu, f, E4M3) << (8 * b);
                     w[e] = o;
                 }
                 *at = v;
@@ -288,28 +298,36 @@ __global__ void __launch_bounds__(kCopyThreads) quantized_copy_kernel(const Quan
     if (wu == 0 && lane == 0) *scale = s;
 
     const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
-    const float half_step = 0.5f * s;
+    const float half_step = s > 0.f ? 0.5f * s : INFINITY;
     for (int q = 0; q < chunks; ++q) {
         if (REREAD) load_rows(q);
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
             const int p = row_of(q, i);
-            if (!col || p < un.p0 || p >= un.p1) continue;
-            float f[16];
-            r[i].unpack(f);
-            uint32_t w[4];
-            float off = 0.f;
+            if (p < un.p0 || p >= un.p1) continue;
+            uint8_t* row = dst + static_cast<int64_t>(p) * a.c_s1[m];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = encode4(f + 4 * e, s, inv, a.e4m3, off);
-            if (odd || s == 0.f || (!a.e4m3 && off >= half_step)) {
+            for (int n = 0; n < Row::N; ++n) {
+                if (Row::col(n, cl) >= a.D) continue;
+                float f[Row::E];
+                unpack16<T>(r[i].v[n], f);
+                uint32_t w[Row::E / 4];
+                float off = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    w[e] = 0;
+                for (int e = 0; e < Row::E / 4; ++e) w[e] = encode4<E4M3>(f + 4 * e, s, inv, off);
+                if (odd || (!E4M3 && off >= half_step)) {
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) w[e] |= encode_slow(f[4 * e + b], s, a.e4m3) << (8 * b);
+                    for (int e = 0; e < Row::E / 4; ++e) {
+                        w[e] = 0;
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) w[e] |= encode_slow<E4M3>(f[4 * e + b], s) << (8 * b);
+                    }
                 }
+                if constexpr (Row::E == 8)
+                    *reinterpret_cast<uint2*>(row + Row::col(n, cl)) = make_uint2(w[0], w[1]);
+                else
+                    *reinterpret_cast<uint32_t*>(row + Row::col(n, cl)) = w[0];
             }
-            *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(p) * a.c_s1[m]) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
 }
@@ -351,21 +369,26 @@ __global__ void __launch_bounds__(kCopyThreads) quantized_copy_any_kernel(const 
     if (tid == 0) *scale = s;
     for (int64_t i = tid; i < n; i += kCopyThreads) {
         const float x = Cvt<T>::to_f(src[i / a.D * a.src_s0[m] + i % a.D * a.src_s2[m]]);
-        dst[(un.p0 + i / a.D) * a.c_s1[m] + i % a.D * a.c_s3[m]] = static_cast<uint8_t>(encode_slow(x, s, a.e4m3));
+        dst[(un.p0 + i / a.D) * a.c_s1[m] + i % a.D * a.c_s3[m]] = static_cast<uint8_t>(a.e4m3 ? encode_slow<true>(x, s) : encode_slow<false>(x, s));
     }
 }
 
-template <typename T, int LPR>
+template <typename T, bool E4M3, int LPR>
 void launch_rows(const QuantCopyArgs& a, int units, cudaStream_t st) {
     auto go = [&](auto kern, int w) {
         const int upc = kCopyWarps / w;
         kern<<<dim3(units, (a.H + upc - 1) / upc, 2), kCopyThreads, 0, st>>>(a);
     };
-    if (a.block_size <= 16) go(quantized_copy_kernel<T, LPR, 1, false>, 1);
-    else if (a.block_size <= 32) go(quantized_copy_kernel<T, LPR, 2, false>, 2);
-    else if (a.block_size <= 64) go(quantized_copy_kernel<T, LPR, 4, false>, 4);
-    else if (a.block_size <= 128) go(quantized_copy_kernel<T, LPR, 8, false>, 8);
-    else go(quantized_copy_kernel<T, LPR, 8, true>, 8);
+    if (a.block_size <= 16) go(quantized_copy_kernel<T, E4M3, LPR, 1, false>, 1);
+    else if (a.block_size <= 32) go(quantized_copy_kernel<T, E4M3, LPR, 2, false>, 2);
+    else if (a.block_size <= 64) go(quantized_copy_kernel<T, E4M3, LPR, 4, false>, 4);
+    else if (a.block_size <= 128) go(quantized_copy_kernel<T, E4M3, LPR, 8, false>, 8);
+    else go(quantized_copy_kernel<T, E4M3, LPR, 8, true>, 8);
+}
+
+template <typename T, int LPR>
+void launch_kind(const QuantCopyArgs& a, int units, cudaStream_t st) {
+    a.e4m3 ? launch_rows<T, true, LPR>(a, units, st) : launch_rows<T, false, LPR>(a, units, st);
 }
 
 template <typename T>
@@ -380,11 +403,11 @@ void launch_t(const QuantCopyArgs& a, int units, cudaStream_t st) {
     if (!rows)
         quantized_copy_any_kernel<T><<<dim3(units, a.H, 2), kCopyThreads, 0, st>>>(a);
     else if (a.D <= 64)
-        launch_rows<T, 4>(a, units, st);
+        launch_kind<T, 4>(a, units, st);
     else if (a.D <= 128)
-        launch_rows<T, 8>(a, units, st);
+        launch_kind<T, 8>(a, units, st);
     else
-        launch_rows<T, 16>(a, units, st);
+        launch_kind<T, 16>(a, units, st);
 }
 
 }  // namespace

@@ -231,6 +231,32 @@ RT_EXPORT diopiTensorHandle_t b200rt_tensor_create(void* data, int ndim, const i
 
 RT_EXPORT void b200rt_tensor_destroy(diopiTensorHandle_t t) { delete t; }
 
+// The handles of one call at once (a call into this library per tensor is what a Python caller spends most of its time on).
+// `desc` holds, one tensor after the other, ndim, dtype, device, data pointer, shape[ndim], stride[ndim]; ndim = -1 alone
+// stands for a null handle. The handles go to `out`; the returned batch is what b200rt_batch_destroy takes.
+RT_EXPORT void* b200rt_batch_create(const int64_t* desc, int n, void** out) {
+    auto* batch = new std::vector<diopiTensor>(static_cast<size_t>(n));
+    for (int i = 0; i < n; ++i) {
+        const int64_t nd = *desc++;
+        out[i] = nullptr;
+        if (nd < 0) continue;
+        diopiTensor& t = (*batch)[i];
+        t.dtype = static_cast<diopiDtype_t>(desc[0]);
+        t.device = static_cast<diopiDevice_t>(desc[1]);
+        t.data = reinterpret_cast<void*>(static_cast<uintptr_t>(desc[2]));
+        desc += 3;
+        t.shape.assign(desc, desc + nd);
+        t.stride.assign(desc + nd, desc + 2 * nd);
+        desc += 2 * nd;
+        t.numel = 1;
+        for (auto s : t.shape) t.numel *= s;
+        out[i] = &t;
+    }
+    return batch;
+}
+
+RT_EXPORT void b200rt_batch_destroy(void* batch) { delete static_cast<std::vector<diopiTensor>*>(batch); }
+
 // stream == nullptr and lazy != 0: the context creates its own stream at first use.
 // stream == nullptr and lazy == 0: the legacy default stream is used.
 RT_EXPORT diopiContextHandle_t b200rt_context_create(void* stream, int lazy) {

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .runtime import Context, Sizes, Tensor, check_returncode, default_context
+from .runtime import Context, Sizes, Tensor, call_with, check_returncode, default_context
 
 
 def _impl():
@@ -30,6 +30,14 @@ def _call(name: str, ctx: Context | None, *args):
     ctx = ctx or default_context()
     rc = getattr(_impl(), name)(ctx.handle, *args)
     check_returncode(name, rc)
+
+
+def _run(name: str, ctx: Context | None, tensors, as_device, *args):
+    """One call whose handles live as long as it does."""
+    ctx = ctx or default_context()
+    rc = call_with(getattr(_impl(), name), ctx.handle, tensors, args, as_device)
+    if rc:
+        check_returncode(name, rc)
 
 
 def vendor_name() -> str:
@@ -118,8 +126,8 @@ def build_block_table(block_table, cached_lens, new_lens, free_blocks, free_star
     blocks from free_blocks[free_start:] in request order, writes their entries of block_table [B, cols], slot_map [T] (the
     slot of each new token; INT32_MIN behind the last), new_start [B + 1], seq_lens [B], free_next [1] and, when given,
     token_table [B, N] (one slot for each token, right-aligned: the b_loc of token_decode_attention). Returns block_table."""
-    ts = [_t(x, as_device) for x in (block_table, slot_map, new_start, seq_lens, token_table, free_next, cached_lens, new_lens, free_blocks, free_start)]
-    _call("diopiBuildBlockTable", ctx, *[_h(t) for t in ts], int(block_size))
+    _run("diopiBuildBlockTable", ctx, (block_table, slot_map, new_start, seq_lens, token_table, free_next, cached_lens, new_lens, free_blocks, free_start), as_device,
+         int(block_size))
     return block_table
 
 
@@ -127,8 +135,7 @@ def quantized_copy_kv(k, v, block_table, cached_lens, new_start, k_cache, v_cach
     """Rows new_start[i] + t of k, v [T, Hkv, D] into positions cached_lens[i] + t of request i of the 8-bit caches
     [blocks, block_size, Hkv, D] (int8, or float8_e4m3fn / uint8 holding its bits), whose scales [blocks, Hkv] start anew with a
     block and grow by powers of two after that. Returns (k_cache, v_cache)."""
-    ts = [_t(x, as_device) for x in (k_cache, v_cache, k_scale, v_scale, k, v, block_table, cached_lens, new_start)]
-    _call("diopiQuantizedCopyKV", ctx, *[_h(t) for t in ts])
+    _run("diopiQuantizedCopyKV", ctx, (k_cache, v_cache, k_scale, v_scale, k, v, block_table, cached_lens, new_start), as_device)
     return k_cache, v_cache
 
 
@@ -137,8 +144,7 @@ def quantized_paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table
     over the 8-bit caches; seq_lens counts all tokens, the new ones among them. Returns out (a new tensor like q)."""
     if out is None:
         out = torch.empty_like(q)
-    ts = [_t(x, as_device) for x in (out, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens)]
-    _call("diopiQuantizedPagedAttention", ctx, *[_h(t) for t in ts], float(softmax_scale))
+    _run("diopiQuantizedPagedAttention", ctx, (out, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens), as_device, float(softmax_scale))
     return out
 
 
