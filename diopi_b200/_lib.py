@@ -1,4 +1,4 @@
-"""Loads the two shared libraries and declares their C signatures for ctypes.
+"""Loads the shared libraries and declares their C signatures for ctypes.
 
 The consumer-side run time (libdiopi_rt.so) is loaded first with RTLD_GLOBAL so that
 the backend (libdiopi_impl.so) resolves diopiGetTensorData, diopiGetStream, ... from
@@ -8,6 +8,8 @@ There is no fallback: a missing library is an error.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 from ctypes import POINTER, c_bool, c_char_p, c_double, c_int, c_int64, c_void_p
 from pathlib import Path
@@ -24,6 +26,8 @@ class diopiSize_t(ctypes.Structure):
 class _Libs:
     rt: ctypes.CDLL | None = None
     impl: ctypes.CDLL | None = None
+    pycall = None          # the module that calls an op with torch tensors; see runtime.call_with
+    address: dict = {}     # op name -> address
 
 
 _libs = _Libs()
@@ -68,7 +72,8 @@ def load() -> _Libs:
         return _libs
     rt_path = LIB_DIR / "libdiopi_rt.so"
     impl_path = LIB_DIR / "libdiopi_impl.so"
-    for p in (rt_path, impl_path):
+    py_path = LIB_DIR / "_pycall.so"
+    for p in (rt_path, impl_path, py_path):
         if not p.exists():
             raise RuntimeError(
                 f"{p} is missing: the CUDA libraries of diopi_b200 are not built "
@@ -81,10 +86,6 @@ def load() -> _Libs:
     rt.b200rt_tensor_create.argtypes = [c_void_p, c_int, POINTER(c_int64), POINTER(c_int64), c_int, c_int]
     rt.b200rt_tensor_destroy.restype = None
     rt.b200rt_tensor_destroy.argtypes = [c_void_p]
-    rt.b200rt_batch_create.restype = c_void_p
-    rt.b200rt_batch_create.argtypes = [c_void_p, c_int, c_void_p]
-    rt.b200rt_batch_destroy.restype = None
-    rt.b200rt_batch_destroy.argtypes = [c_void_p]
     rt.b200rt_context_create.restype = c_void_p
     rt.b200rt_context_create.argtypes = [c_void_p, c_int]
     rt.b200rt_context_set_stream.restype = None
@@ -110,5 +111,9 @@ def load() -> _Libs:
         fn = getattr(impl, name)
         fn.restype = c_char_p
         fn.argtypes = []
-    _libs.rt, _libs.impl = rt, impl
+    loader = importlib.machinery.ExtensionFileLoader("_pycall", str(py_path))
+    pycall = importlib.util.module_from_spec(importlib.util.spec_from_loader("_pycall", loader))
+    loader.exec_module(pycall)
+    _libs.address = {name: ctypes.cast(getattr(impl, name), c_void_p).value for name in OPS}
+    _libs.rt, _libs.impl, _libs.pycall = rt, impl, pycall
     return _libs

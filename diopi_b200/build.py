@@ -1,7 +1,8 @@
-"""Builds the two shared libraries of the package with nvcc, in-tree.
+"""Builds the shared libraries of the package with nvcc, in-tree.
 
   diopi_b200/lib/libdiopi_impl.so  the backend: exported DIOPI ops + sm_100a kernels
   diopi_b200/lib/libdiopi_rt.so    the consumer-side test run time (tensor/context handles)
+  diopi_b200/lib/_pycall.so        the CPython module that makes one op call from torch tensors
 
 The backend leaves the diopirt accessors (diopiGetTensorData, diopiGetStream, ...)
 undefined, as a DIOPI backend does (impl/CMakeLists.txt:45-46 builds one
@@ -15,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -50,6 +52,7 @@ IMPL_SOURCES = [
     "kernels/quantized_attention.cu",
 ]
 RT_SOURCES = ["rt/testrt.cpp"]
+PY_SOURCES = ["rt/pycall.cpp"]
 
 
 def nvcc() -> str:
@@ -75,6 +78,8 @@ def _compile(src: str, stamp: str, verbose: bool) -> Path:
     for old in OBJ.glob(src.replace("/", "_") + ".*.o"):
         old.unlink()
     cmd = [nvcc(), "-x", "cu", *ARCH, *COMMON, "-c", str(s), "-o", str(o)]
+    if src in PY_SOURCES:
+        cmd.insert(1, f"-I{sysconfig.get_paths()['include']}")
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -94,33 +99,36 @@ def _link(objs: list[Path], out: Path, extra: list[str]) -> None:
 
 def _sources_stamp() -> str:
     h = hashlib.sha1(_headers_stamp().encode())
-    for src in IMPL_SOURCES + RT_SOURCES:
+    for src in IMPL_SOURCES + RT_SOURCES + PY_SOURCES:
         h.update((CSRC / src).read_bytes())
     return h.hexdigest()
 
 
 def build(verbose: bool = False, jobs: int | None = None) -> dict[str, Path]:
-    """Compiles what is out of date and returns the paths of the two libraries.
+    """Compiles what is out of date and returns the paths of the libraries.
 
     lib/build_stamp.txt holds a hash of every source, header and flag the libraries were built from;
     when it matches, nothing is compiled (file times do not survive a copy of the tree, hashes do)."""
     LIB.mkdir(parents=True, exist_ok=True)
     impl = LIB / "libdiopi_impl.so"
     rt = LIB / "libdiopi_rt.so"
+    py = LIB / "_pycall.so"
     stamp_file = LIB / "build_stamp.txt"
     full = _sources_stamp()
-    if not verbose and impl.exists() and rt.exists() and stamp_file.exists() and stamp_file.read_text().strip() == full:
-        return {"impl": impl, "rt": rt}
+    if not verbose and impl.exists() and rt.exists() and py.exists() and stamp_file.exists() and stamp_file.read_text().strip() == full:
+        return {"impl": impl, "rt": rt, "py": py}
     OBJ.mkdir(parents=True, exist_ok=True)
     stamp = _headers_stamp()
     jobs = jobs or min(8, os.cpu_count() or 1)
     with ThreadPoolExecutor(jobs) as ex:
         impl_objs = list(ex.map(lambda s: _compile(s, stamp, verbose), IMPL_SOURCES))
         rt_objs = list(ex.map(lambda s: _compile(s, stamp, verbose), RT_SOURCES))
+        py_objs = list(ex.map(lambda s: _compile(s, stamp, verbose), PY_SOURCES))
     _link(impl_objs, impl, [])
     _link(rt_objs, rt, [])
+    _link(py_objs, py, [])
     stamp_file.write_text(full + "\n")
-    return {"impl": impl, "rt": rt}
+    return {"impl": impl, "rt": rt, "py": py}
 
 
 if __name__ == "__main__":

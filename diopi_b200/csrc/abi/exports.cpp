@@ -1162,9 +1162,9 @@ B200_EXPORT diopiError_t diopiQuantizedCopyKV(diopiContextHandle_t ctx, diopiTen
         a.blocks = c.blocks;
         if (B == 0 || a.T == 0) return;
         cudaStream_t st = stream_of(ctx);
-        device_info();
+        const DeviceInfo& di = device_info();
         a.status = async_status_device_ptr();
-        k::launch_quantized_copy_kv(a, st);
+        k::launch_quantized_copy_kv(a, di.sm_count, st);
         B200_CUDA(cudaGetLastError());
     });
 }

@@ -42,7 +42,7 @@ __device__ __forceinline__ RequestSpan span_of(const BlockTableArgs& a, int i) {
     return s;
 }
 
-__global__ void __launch_bounds__(kTableThreads) block_table_kernel(const BlockTableArgs a) {
+__global__ void __launch_bounds__(kTableThreads, 6) block_table_kernel(const BlockTableArgs a) {
     __shared__ int64_t part[2][kTableThreads / 32];
     const int i = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int bs = a.block_size;
@@ -101,16 +101,13 @@ __global__ void __launch_bounds__(kTableThreads) block_table_kernel(const BlockT
         }
     }
 
-    // The slot of position p: kNoSlot where there is no block, or where the slot does not fit the tensor's type.
-    auto slot_of = [&](uint32_t p, int is64) -> int64_t {
-        const uint32_t b = p / static_cast<uint32_t>(bs), o = p - b * static_cast<uint32_t>(bs);
-        int64_t id;
-        if (b < have) {
-            id = load_index(a.table, i, b);
-        } else {
-            const int64_t f = first + (b - have);
-            id = f < a.n_free ? load_index(a.free_blocks, f) : -1;
-        }
+    auto block_id = [&](uint32_t b) -> int64_t {
+        if (b < have) return load_index(a.table, i, b);
+        const int64_t f = first + (b - have);
+        return f < a.n_free ? load_index(a.free_blocks, f) : -1;
+    };
+    // The slot at offset o of a block: kNoSlot where there is no block, or where the slot does not fit the tensor's type.
+    auto slot_in = [&](int64_t id, uint32_t o, bool is64) -> int64_t {
         const int64_t slot = id * bs + o;
         if (id < 0 || (!is64 && slot > 0x7fffffffll)) {
             bad = true;
@@ -118,22 +115,52 @@ __global__ void __launch_bounds__(kTableThreads) block_table_kernel(const BlockT
         }
         return slot;
     };
-
-    const int64_t stride = static_cast<int64_t>(gridDim.y) * kTableThreads, at = static_cast<int64_t>(blockIdx.y) * kTableThreads + tid;
-    for (int64_t t = at; t < s.raw; t += stride) {
-        if (before + t >= a.T) {
-            bad = true;
-            break;
+    const uint32_t stride = gridDim.y * kTableThreads, at = blockIdx.y * kTableThreads + tid;
+    // The slots of positions pos .. pos + n - 1 to n elements of `to`, `step` apart from element `off` on.
+    auto write_slots = [&](const IndexArg& to, int64_t off, int64_t step, int64_t n, uint32_t pos) {
+        if (step == 1 && !to.is64) {
+            // four at a time, one division and one block id for them unless a block ends among them
+            int32_t* d = static_cast<int32_t*>(const_cast<void*>(to.ptr)) + off;
+            const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(d) / 4 % 4);   // elements of the first aligned four that are not ours
+            for (int64_t k = 4ll * at - lead; k < n; k += 4ll * stride) {
+                const int e0 = k < 0 ? static_cast<int>(-k) : 0, e1 = n - k < 4 ? static_cast<int>(n - k) : 4;
+                const uint32_t p = pos + static_cast<uint32_t>(k + e0);
+                uint32_t b = p / static_cast<uint32_t>(bs), o = p - b * static_cast<uint32_t>(bs);
+                int64_t id = block_id(b);
+                int32_t v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = 0;
+                    if (e < e0 || e >= e1) continue;
+                    if (o == static_cast<uint32_t>(bs)) {
+                        id = block_id(++b);
+                        o = 0;
+                    }
+                    v[e] = static_cast<int32_t>(slot_in(id, o++, false));
+                }
+                if (e0 == 0 && e1 == 4) {
+                    *reinterpret_cast<int4*>(d + k) = make_int4(v[0], v[1], v[2], v[3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e >= e0 && e < e1) d[k + e] = v[e];
+                }
+            }
+            return;
         }
-        const int64_t v = t < s.n ? slot_of(static_cast<uint32_t>(s.c + t), a.slot_map.is64) : static_cast<int64_t>(kNoSlot);
-        store_index(a.slot_map, (before + t) * a.slot_map.s0, v);
-    }
+        for (int64_t k = at; k < n; k += stride) {
+            const uint32_t p = pos + static_cast<uint32_t>(k), b = p / static_cast<uint32_t>(bs);
+            store_index(to, off + k * step, slot_in(block_id(b), p - b * static_cast<uint32_t>(bs), to.is64));
+        }
+    };
+    const int64_t room = imax64(imin64(s.raw, a.T - before), 0);   // new tokens that slot_map has entries for
+    if (room < s.raw) bad = true;
+    write_slots(a.slot_map, before * a.slot_map.s0, a.slot_map.s0, imin64(room, s.n), static_cast<uint32_t>(s.c));
+    for (int64_t t = s.n + at; t < room; t += stride) store_index(a.slot_map, (before + t) * a.slot_map.s0, kNoSlot);
     if (a.wide.ptr != nullptr) {
-        const int64_t L = s.c + s.n;
-        if (L > a.wide_cols) bad = true;
-        const int64_t shift = a.wide_cols - L;   // column of position 0
-        for (int64_t p = imax64(-shift, 0) + at; p < L; p += stride)
-            store_index(a.wide, static_cast<int64_t>(i) * a.wide.s0 + (shift + p) * a.wide.s1, slot_of(static_cast<uint32_t>(p), a.wide.is64));
+        const int64_t L = s.c + s.n, skip = imax64(L - a.wide_cols, 0);   // only the last tokens of a request longer than the row
+        if (skip > 0) bad = true;
+        write_slots(a.wide, static_cast<int64_t>(i) * a.wide.s0 + (a.wide_cols - L + skip) * a.wide.s1, a.wide.s1, L - skip, static_cast<uint32_t>(skip));
     }
     if (bad || ran_out) report_status(a.status, 4);
 }

@@ -98,7 +98,7 @@ struct QuantCopyArgs {
     int64_t T, blocks;
     int* status;
 };
-void launch_quantized_copy_kv(const QuantCopyArgs& a, cudaStream_t st);
+void launch_quantized_copy_kv(const QuantCopyArgs& a, int sm_count, cudaStream_t st);
 
 struct QuantAttnArgs {
     Dt dt;                                               // of q and out

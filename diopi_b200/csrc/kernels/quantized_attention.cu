@@ -135,7 +135,7 @@ constexpr int kTilesPerRange = 4;               // at least, so that short batch
 
 // Warps of a CTA: as many as the registers of a thread's queries and accumulators leave room for (a spilled register costs
 // an L2 access here, as shared memory leaves no L1).
-constexpr int split_warps(bool f32, int hd, int nt) { return hd > 128 || nt > 1 ? 8 : f32 ? 12 : 16; }
+constexpr int split_warps(bool f32, int hd, int nt) { return hd * nt * (f32 ? 2 : 1) <= 128 ? 16 : hd == 128 && f32 ? 12 : 8; }
 
 struct QuantPlan {
     int hd;           // 64, 128 or 256: head_dim rounded up
@@ -218,6 +218,8 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
     volatile int* give_up = reinterpret_cast<volatile int*>(smem + p.off_flag);
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x < 2)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(threadIdx.x == 0 ? &map_k : &map_v)) : "memory");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = a.Hq / a.Hkv;
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
     const int hl = team % p.hw, range = blockIdx.x * p.tw + team / p.hw;
     const int total = pre[a.B];
     const int used = used_ranges(total, p.n_range);
-    if (team < teams && range < used) {
+    if (team < teams && range < used && total > 0) {
         const int t0 = static_cast<int>(static_cast<int64_t>(total) * range / used);
         const int t1 = static_cast<int>(static_cast<int64_t>(total) * (range + 1) / used);
         const int hkv = blockIdx.y * p.hw + hl;
@@ -283,20 +285,22 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
             }
             return lo;
         };
-        auto load_ids = [&](Ahead& x, int base) {
-            x.block = 0;
+        // In two halves, so that what comes between them hides the load of the block ids.
+        auto ask_ids = [&](Ahead& x, int from) -> int64_t {
             x.at = 0;
+            const int t = from + lane;
+            if (t >= t1) return 0;
+            const int i = request_of(t);
+            const int pos = (t - pre[i]) * kTile, col = pos / a.block_size;
+            x.at = (pos - col * a.block_size) * 32 + min(kTile, lens[i] - pos);
+            return load_index(a.table, i, col);
+        };
+        auto take_ids = [&](Ahead& x, int64_t id) {
+            const bool ok = id >= 0 && id < a.blocks;
+            if (!ok) report_status(a.status, 1);
+            x.block = ok ? static_cast<int>(id) : 0;
+            if (!ok) x.at = 0;
             x.ks = x.vs = 0.f;
-            const int t = base + lane;
-            if (t < t1) {
-                const int i = request_of(t);
-                const int pos = (t - pre[i]) * kTile, col = pos / a.block_size;
-                const int64_t id = load_index(a.table, i, col);
-                const bool ok = id >= 0 && id < a.blocks;
-                if (!ok) report_status(a.status, 1);
-                x.block = ok ? static_cast<int>(id) : 0;
-                x.at = ok ? (pos - col * a.block_size) * 32 + min(kTile, lens[i] - pos) : 0;
-            }
         };
         auto load_scales = [&](Ahead& x) {
             if (x.at != 0) {
@@ -317,17 +321,6 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                 tma_4d(dst + (NH + h) * BOX, &map_v, h * RB, at >> 5, hkv, block, full);
             }
         };
-        int base = t0;
-        load_ids(cur, base);
-        load_scales(cur);
-        if (mtile == 0) {
-            for (int k = 0; k < min(p.stages, t1 - t0); ++k) {
-                const int block = __shfl_sync(0xffffffffu, cur.block, k), at = __shfl_sync(0xffffffffu, cur.at, k);
-                if (lane == 0) fetch(k, block, at);
-            }
-        }
-        load_ids(nxt, base + 32);
-
         const int g = lane >> 2, c = lane & 3;
         const int rbase = (blockIdx.z * p.mt + mtile) * 8 * NT;   // first query row of this warp
         // K: lane l names row l & 7 of matrix l >> 3, matrix m being the 16 bytes 4 i + m of eight tokens. In each register the lane
@@ -341,6 +334,111 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
         float o[NT][DM][4];                             // rows 2c (elements 0, 2) and 2c + 1 (1, 3) of the N tile
         float ref[NT][2], l[NT][2], rs[NT][2];
         int req = request_of(t0) - 1, req_end = t0, part_first = 0, lim_min = 0;
+        // The next request from tile t on: its query rows as they are in memory ...
+        auto ask_request = [&](int t) {
+            do ++req;
+            while (pre[req + 1] <= t);
+            req_end = min(pre[req + 1], t1);
+            part_first = t - pre[req];
+            lim_min = lens[req] - (a.n - 1);            // what the first new token sees
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                // ---- query row g of the N tile as a B fragment ----
+                const int r = rbase + 8 * n + g, tq = r / group;
+                const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(req) * a.q_s0 + static_cast<int64_t>(tq) * a.q_s1 +
+                             static_cast<int64_t>(hkv * group + (r - tq * group)) * a.q_s2 + 4 * c;
+                const int dmax = r < R ? a.D - 4 * c : 0;
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int i = 0; i < CH; ++i) {
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (16 * i < dmax) v = p.qvec ? *reinterpret_cast<const float4*>(q + 16 * i) : make_float4(q[16 * i], q[16 * i + 1], q[16 * i + 2], q[16 * i + 3]);
+                        qf[n][i][0] = __float_as_uint(v.x);
+                        qf[n][i][1] = __float_as_uint(v.y);
+                        ql[n][i][0] = __float_as_uint(v.z);
+                        ql[n][i][1] = __float_as_uint(v.w);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < CH; ++i) {
+                        uint2 v = make_uint2(0u, 0u);
+                        if (16 * i < dmax) {
+                            const unsigned short* e = reinterpret_cast<const unsigned short*>(q + 16 * i);
+                            if (p.qvec)
+                                v = *reinterpret_cast<const uint2*>(e);
+                            else
+                                v = make_uint2(e[0] | (static_cast<uint32_t>(e[1]) << 16), e[2] | (static_cast<uint32_t>(e[3]) << 16));
+                        }
+                        qf[n][i][0] = v.x;
+                        qf[n][i][1] = v.y;
+                    }
+                }
+            }
+        };
+        // ... and as B fragments: row g of each N tile.
+        auto take_request = [&] {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float scale = 1.f, back = 1.f;
+                if constexpr (!std::is_same<T, __half>::value) {   // 2^-e with the row's maximum in [2^e, 2^(e + 1))
+                    float amax = 0.f;
+#pragma unroll
+                    for (int i = 0; i < CH; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t u = qf[n][i][h];
+                            if constexpr (SPLIT)
+                                amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(u)), fabsf(__uint_as_float(ql[n][i][h]))));
+                            else
+                                amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(u << 16)), fabsf(__uint_as_float(u & 0xffff0000u))));
+                        }
+                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                    const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
+                    scale = __uint_as_float((254u - e) << 23);
+                    back = __uint_as_float(e << 23);
+#pragma unroll
+                    for (int i = 0; i < CH; ++i) {
+                        if constexpr (SPLIT) {
+                            const float x0 = __uint_as_float(qf[n][i][0]) * scale, x1 = __uint_as_float(qf[n][i][1]) * scale;
+                            const float x2 = __uint_as_float(ql[n][i][0]) * scale, x3 = __uint_as_float(ql[n][i][1]) * scale;
+                            qf[n][i][0] = pack_f16(x0, x1);
+                            qf[n][i][1] = pack_f16(x2, x3);
+                            ql[n][i][0] = pack_rest(x0, x1, qf[n][i][0]);
+                            ql[n][i][1] = pack_rest(x2, x3, qf[n][i][1]);
+                        } else {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                qf[n][i][h] = pack_f16(__uint_as_float(qf[n][i][h] << 16) * scale, __uint_as_float(qf[n][i][h] & 0xffff0000u) * scale);
+                        }
+                    }
+                }
+                back *= a.softmax_scale * kLog2e;
+                rs[n][0] = __shfl_sync(0xffffffffu, back, 8 * c);       // of row 2c
+                rs[n][1] = __shfl_sync(0xffffffffu, back, 8 * c + 4);   // of row 2c + 1
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    ref[n][e] = -INFINITY;
+                    l[n][e] = 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < DM; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+            }
+        };
+
+        int base = t0;
+        const int64_t ids = ask_ids(cur, base);
+        ask_request(t0);
+        take_ids(cur, ids);
+        load_scales(cur);
+        if (mtile == 0) {
+            for (int k = 0; k < min(p.stages, t1 - t0); ++k)
+                if (lane == k) fetch(k, cur.block, cur.at);
+        }
+        __syncwarp();
+        take_ids(nxt, ask_ids(nxt, base + 32));
+        take_request();
+
         int slot = 0;
         uint32_t phase = 0;
         for (int t = t0; t < t1; ++t) {
@@ -349,87 +447,12 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                 cur = nxt;
                 base += 32;
                 k = 0;
-                load_ids(nxt, base + 32);
+                take_ids(nxt, ask_ids(nxt, base + 32));
             }
             if (k == 16) load_scales(nxt);
             if (t == req_end) {
-                do ++req;
-                while (pre[req + 1] <= t);
-                req_end = min(pre[req + 1], t1);
-                part_first = t - pre[req];
-                lim_min = lens[req] - (a.n - 1);            // what the first new token sees
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    // ---- query row g of the N tile as a B fragment ----
-                    const int r = rbase + 8 * n + g, tq = r / group;
-                    const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(req) * a.q_s0 + static_cast<int64_t>(tq) * a.q_s1 +
-                                 static_cast<int64_t>(hkv * group + (r - tq * group)) * a.q_s2 + 4 * c;
-                    const int dmax = r < R ? a.D - 4 * c : 0;
-                    float amax = 0.f, scale = 1.f, back = 1.f;
-                    if constexpr (SPLIT) {
-#pragma unroll
-                        for (int i = 0; i < CH; ++i) {
-                            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (16 * i < dmax) v = p.qvec ? *reinterpret_cast<const float4*>(q + 16 * i) : make_float4(q[16 * i], q[16 * i + 1], q[16 * i + 2], q[16 * i + 3]);
-                            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-                            qf[n][i][0] = __float_as_uint(v.x);
-                            qf[n][i][1] = __float_as_uint(v.y);
-                            ql[n][i][0] = __float_as_uint(v.z);
-                            ql[n][i][1] = __float_as_uint(v.w);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < CH; ++i) {
-                            uint2 v = make_uint2(0u, 0u);
-                            if (16 * i < dmax) {
-                                const unsigned short* e = reinterpret_cast<const unsigned short*>(q + 16 * i);
-                                if (p.qvec)
-                                    v = *reinterpret_cast<const uint2*>(e);
-                                else
-                                    v = make_uint2(e[0] | (static_cast<uint32_t>(e[1]) << 16), e[2] | (static_cast<uint32_t>(e[3]) << 16));
-                            }
-                            qf[n][i][0] = v.x;
-                            qf[n][i][1] = v.y;
-                            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-#pragma unroll
-                                for (int h = 0; h < 2; ++h)
-                                    amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(qf[n][i][h] << 16)), fabsf(__uint_as_float(qf[n][i][h] & 0xffff0000u))));
-                            }
-                        }
-                    }
-                    if constexpr (!std::is_same<T, __half>::value) {   // 2^-e with the row's maximum in [2^e, 2^(e + 1))
-                        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                        const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
-                        scale = __uint_as_float((254u - e) << 23);
-                        back = __uint_as_float(e << 23);
-#pragma unroll
-                        for (int i = 0; i < CH; ++i) {
-                            if constexpr (SPLIT) {
-                                const float x0 = __uint_as_float(qf[n][i][0]) * scale, x1 = __uint_as_float(qf[n][i][1]) * scale;
-                                const float x2 = __uint_as_float(ql[n][i][0]) * scale, x3 = __uint_as_float(ql[n][i][1]) * scale;
-                                qf[n][i][0] = pack_f16(x0, x1);
-                                qf[n][i][1] = pack_f16(x2, x3);
-                                ql[n][i][0] = pack_rest(x0, x1, qf[n][i][0]);
-                                ql[n][i][1] = pack_rest(x2, x3, qf[n][i][1]);
-                            } else {
-#pragma unroll
-                                for (int h = 0; h < 2; ++h)
-                                    qf[n][i][h] = pack_f16(__uint_as_float(qf[n][i][h] << 16) * scale, __uint_as_float(qf[n][i][h] & 0xffff0000u) * scale);
-                            }
-                        }
-                    }
-                    back *= a.softmax_scale * kLog2e;
-                    rs[n][0] = __shfl_sync(0xffffffffu, back, 8 * c);       // of row 2c
-                    rs[n][1] = __shfl_sync(0xffffffffu, back, 8 * c + 4);   // of row 2c + 1
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        ref[n][e] = -INFINITY;
-                        l[n][e] = 0.f;
-                    }
-#pragma unroll
-                    for (int j = 0; j < DM; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
-                }
+                ask_request(t);
+                take_request();
             }
             const int valid = __shfl_sync(0xffffffffu, cur.at, k) & 31;
             const float ks = __shfl_sync(0xffffffffu, cur.ks, k), vs = __shfl_sync(0xffffffffu, cur.vs, k);
@@ -458,6 +481,37 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                             if constexpr (SPLIT) mma_f16(s[n], f, ql[n][i + m][0], ql[n][i + m][1]);
                         }
                     }
+                }
+                // ---- the codes of V, on their way while the weights are made ----
+                uint32_t v[NH][4][VB / 4];   // tokens 2c, 2c + 1, 2c + 8, 2c + 9
+#pragma unroll
+                for (int h = 0; h < NH; ++h) {
+                    const uint32_t vb = kt + h * BOX + v_lane;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t trow = (i & 1) * RB + (i >> 1) * 8 * RB;
+                        if constexpr (RB == 128) {
+                            const uint32_t at = vb + trow + ((g ^ (2 * c + (i & 1))) << 4);
+                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(v[h][i][0]), "=r"(v[h][i][1]), "=r"(v[h][i][2]), "=r"(v[h][i][3])
+                                         : "r"(at)
+                                         : "memory");
+                        } else {
+                            const uint32_t at = vb + trow + (((g >> 1) ^ c) << 4) + (g & 1) * 8;
+                            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[h][i][0]), "=r"(v[h][i][1]) : "r"(at) : "memory");
+                        }
+                    }
+                }
+                // Codes of tokens that do not exist are whatever the block holds, NaN perhaps: their weight is 0, so are they.
+                if (valid < kTile) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (2 * c + (i & 1) + (i >> 1) * 8 >= valid) {
+#pragma unroll
+                            for (int h = 0; h < NH; ++h)
+#pragma unroll
+                                for (int w = 0; w < VB / 4; ++w) v[h][i][w] = 0u;
+                        }
                 }
                 // ---- weights against the tile's own maximum ----
                 // s[0], s[1]: token g, rows 2c, 2c + 1; s[2], s[3]: token g + 8
@@ -517,35 +571,16 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                     }
                 }
                 // ---- O^T += (w vs) (Vc^T P^T) ----
-                // Codes of tokens that do not exist are whatever the block holds, NaN perhaps: their weight is 0, so are they.
-                uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-                if (valid < kTile) {
-                    keep0 = (2 * c < valid ? 0x00ff00ffu : 0u) | (2 * c + 1 < valid ? 0xff00ff00u : 0u);
-                    keep1 = (2 * c + 8 < valid ? 0x00ff00ffu : 0u) | (2 * c + 9 < valid ? 0xff00ff00u : 0u);
-                }
 #pragma unroll
                 for (int h = 0; h < NH; ++h) {
-                    uint32_t v[4][VB / 4];   // tokens 2c, 2c + 1, 2c + 8, 2c + 9
-                    const uint32_t vb = kt + h * BOX + v_lane;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t trow = (i & 1) * RB + (i >> 1) * 8 * RB;
-                        if constexpr (RB == 128) {
-                            const uint32_t at = vb + trow + ((g ^ (2 * c + (i & 1))) << 4);
-                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[i][0]), "=r"(v[i][1]), "=r"(v[i][2]), "=r"(v[i][3]) : "r"(at) : "memory");
-                        } else {
-                            const uint32_t at = vb + trow + (((g >> 1) ^ c) << 4) + (g & 1) * 8;
-                            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[i][0]), "=r"(v[i][1]) : "r"(at) : "memory");
-                        }
-                    }
 #pragma unroll
                     for (int w = 0; w < VB / 4; ++w) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const uint32_t sel = i == 0 ? 0x5140 : 0x7362;
                             uint32_t f[4];
-                            codes_to_f16<E4M3>(__byte_perm(v[0][w], v[1][w], sel) & keep0, f[0], f[1]);
-                            codes_to_f16<E4M3>(__byte_perm(v[2][w], v[3][w], sel) & keep1, f[2], f[3]);
+                            codes_to_f16<E4M3>(__byte_perm(v[h][0][w], v[h][1][w], sel), f[0], f[1]);
+                            codes_to_f16<E4M3>(__byte_perm(v[h][2][w], v[h][3][w], sel), f[2], f[3]);
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
                                 float (&oj)[4] = o[n][h * (VB / 2) + w * 2 + i];
@@ -570,12 +605,10 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                 const int u = t - lag + p.stages;   // the tile to fetch
                 if (t - lag >= t0 && u < t1) {
                     const int ku = u - base;
-                    const int from_block = ku < 32 ? cur.block : nxt.block, from_at = ku < 32 ? cur.at : nxt.at;
-                    const int block = __shfl_sync(0xffffffffu, from_block, ku & 31), at = __shfl_sync(0xffffffffu, from_at, ku & 31);
                     const int to = slot >= lag ? slot - lag : p.stages - 1;
-                    if (lane == 0) {
+                    if (lane == (ku & 31)) {   // the lane that knows the tile
                         const uint32_t ph = to > slot ? phase ^ 1u : phase;   // the slot before slot 0 was read in the round before
-                        if (lag == 0 || mbar_wait(empty0 + 8u * to, ph, give_up)) fetch(to, block, at);
+                        if (lag == 0 || mbar_wait(empty0 + 8u * to, ph, give_up)) fetch(to, ku < 32 ? cur.block : nxt.block, ku < 32 ? cur.at : nxt.at);
                     }
                     __syncwarp();
                 }
@@ -651,11 +684,12 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
 // read one after the other (four requests of 30011 to 131072 tokens: 145 us with one warp to a row, 5 us with eight).
 constexpr int kMergeWarps = 8;
 
-template <typename T>
-__global__ void __launch_bounds__(32 * kMergeWarps) quant_combine_kernel(const QuantAttnArgs a, int n_range, int wpr, const float* __restrict__ ws_acc,
+template <typename T, bool WIDE>   // WIDE: head_dim above 128
+__global__ void __launch_bounds__(32 * kMergeWarps, WIDE ? 3 : 4) quant_combine_kernel(const QuantAttnArgs a, int n_range, int wpr, const float* __restrict__ ws_acc,
                                                                          const float* __restrict__ ws_ml) {
     __shared__ int s_part[kMergeWarps][2];
-    __shared__ float s_acc[kMergeWarps][32 * 8 + 1];
+    constexpr int NV = WIDE ? 8 : 4;
+    __shared__ float s_acc[kMergeWarps][32 * NV + 1];
     const int i = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int before = 0, all = 0;
     for (int r = threadIdx.x; r < a.B; r += 32 * kMergeWarps) {
@@ -698,9 +732,9 @@ __global__ void __launch_bounds__(32 * kMergeWarps) quant_combine_kernel(const Q
     const int64_t rows = static_cast<int64_t>(a.n) * a.Hq;
     const float* ml = ws_ml + ((static_cast<int64_t>(c_first) + i) * rows + row) * 2;
     const float* acc = ws_acc + ((static_cast<int64_t>(c_first) + i) * rows + row) * a.D;
-    float v[8];   // d = 4 * lane .. + 3, and 128 further
+    float v[NV];   // d = 4 * lane .. + 3, and 128 further
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    for (int e = 0; e < NV; ++e) v[e] = 0.f;
     float L = 0.f;
     if (here) {
         float M = -1e30f;
@@ -710,14 +744,14 @@ __global__ void __launch_bounds__(32 * kMergeWarps) quant_combine_kernel(const Q
         const bool d0 = 4 * lane < a.D, d1 = 4 * lane + 128 < a.D;
         for (int c = sub; c < parts; c += 4 * wpr) {
             float2 x[4];
-            float4 y[4], z[4];
+            float4 y[4], z[WIDE ? 4 : 1];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int64_t at = (c + u * wpr) * rows;
                 const bool in = c + u * wpr < parts;
                 x[u] = in ? *reinterpret_cast<const float2*>(ml + at * 2) : make_float2(-INFINITY, 0.f);
                 y[u] = in && d0 ? *reinterpret_cast<const float4*>(acc + at * a.D + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-                z[u] = in && d1 ? *reinterpret_cast<const float4*>(acc + at * a.D + 4 * lane + 128) : make_float4(0.f, 0.f, 0.f, 0.f);
+                if constexpr (WIDE) z[u] = in && d1 ? *reinterpret_cast<const float4*>(acc + at * a.D + 4 * lane + 128) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -727,23 +761,25 @@ __global__ void __launch_bounds__(32 * kMergeWarps) quant_combine_kernel(const Q
                 v[1] = fmaf(y[u].y, w, v[1]);
                 v[2] = fmaf(y[u].z, w, v[2]);
                 v[3] = fmaf(y[u].w, w, v[3]);
-                v[4] = fmaf(z[u].x, w, v[4]);
-                v[5] = fmaf(z[u].y, w, v[5]);
-                v[6] = fmaf(z[u].z, w, v[6]);
-                v[7] = fmaf(z[u].w, w, v[7]);
+                if constexpr (WIDE) {
+                    v[4] = fmaf(z[u].x, w, v[4]);
+                    v[5] = fmaf(z[u].y, w, v[5]);
+                    v[6] = fmaf(z[u].z, w, v[6]);
+                    v[7] = fmaf(z[u].w, w, v[7]);
+                }
             }
         }
     }
     if (wpr > 1) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s_acc[warp][e * 32 + lane] = v[e];
-        if (lane == 0) s_acc[warp][256] = L;
+        for (int e = 0; e < NV; ++e) s_acc[warp][e * 32 + lane] = v[e];
+        if (lane == 0) s_acc[warp][32 * NV] = L;
         __syncthreads();
         if (sub != 0) return;
         for (int w = 1; w < wpr; ++w) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += s_acc[warp + w][e * 32 + lane];
-            L += s_acc[warp + w][256];
+            for (int e = 0; e < NV; ++e) v[e] += s_acc[warp + w][e * 32 + lane];
+            L += s_acc[warp + w][32 * NV];
         }
     }
     if (!here) return;
@@ -751,7 +787,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) quant_combine_kernel(const Q
     const int t = row / a.Hq, h = row - t * a.Hq;
     T* out = static_cast<T*>(a.out) + static_cast<int64_t>(i) * a.o_s0 + static_cast<int64_t>(t) * a.o_s1 + static_cast<int64_t>(h) * a.o_s2;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < NV; ++e) {
         const int d = 4 * lane + (e & 3) + (e >> 2) * 128;
         if (d < a.D) out[d] = Cvt<T>::from_f(v[e] * inv);
     }
@@ -862,7 +898,7 @@ void launch_split(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap&
     }
     kern<<<dim3(p.n_cta, p.n_hg, p.n_z), threads, p.smem_bytes, st>>>(a, p, mk, mv, acc, ml);
     int wpr = 1;
-    while (wpr < kMergeWarps && wpr * 4 * a.B < p.n_range) wpr *= 2;   // parts of a request on average, four to a warp
+    while (wpr < kMergeWarps && wpr * 8 * a.B < p.n_range) wpr *= 2;   // eight parts to a warp on average
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.B, (a.n * a.Hq + kMergeWarps / wpr - 1) / (kMergeWarps / wpr), 1);
     cfg.blockDim = dim3(32 * kMergeWarps);
@@ -872,7 +908,7 @@ void launch_split(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap&
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, quant_combine_kernel<T>, a, p.n_range, wpr, static_cast<const float*>(acc), static_cast<const float*>(ml));
+    cudaLaunchKernelEx(&cfg, HD > 128 ? quant_combine_kernel<T, true> : quant_combine_kernel<T, false>, a, p.n_range, wpr, static_cast<const float*>(acc), static_cast<const float*>(ml));
 }
 
 template <typename T>

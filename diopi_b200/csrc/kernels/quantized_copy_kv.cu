@@ -71,21 +71,45 @@ __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
     return r;
 }
 
-// Four codes. `inv` = 1 / s (exact for the powers of two of e4m3). int8: adding 1.5 * 2^23 rounds x * inv to an integer,
-// which sits in the low byte; x * inv carries the error of inv, so where the remainder x - q * s (exact in one fma: |q| <=
-// 127) is half a step or more the nearest code may be another one and `off` asks for the slow path.
+// Four codes. e4m3: 1 / s is a power of two, so x * lo is exact (hi is not used). int8: adding 1.5 * 2^23 rounds x * inv to an
+// integer, which sits in the low byte. `lo` and `hi` hold 1 / s between them (the approximate reciprocal is off by one unit
+// in the last place at most), so where both give one code the quotient has it; `split` collects the bits in which they differ.
+struct Inverse {
+    float lo, hi;
+};
 template <bool E4M3>
-__device__ __forceinline__ uint32_t encode4(const float* x, float s, float inv, float& off) {
-    if (E4M3) return e4m3_pair(x[0] * inv, x[1] * inv) | (e4m3_pair(x[2] * inv, x[3] * inv) << 16);
-    constexpr float kMagic = 12582912.f;
-    uint32_t b[4];
+__device__ __forceinline__ Inverse inverse_of(float s) {
+    const uint32_t u = __float_as_uint(s);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+    if (E4M3 && (u & 0x7fffffu) == 0) r = __uint_as_float(0x7f000000u - u);   // 2^-k of 2^k
+    Inverse v;
+    v.lo = s > 0.f ? (E4M3 ? r : __uint_as_float(__float_as_uint(r) - 2)) : 0.f;
+    v.hi = s > 0.f ? (E4M3 ? r : __uint_as_float(__float_as_uint(r) + 2)) : 0.f;
+    return v;
+}
+constexpr float kMagic = 12582912.f;
+template <bool E4M3>
+__device__ __forceinline__ uint32_t encode4(const float* x, Inverse inv, uint32_t& split) {
+    if constexpr (E4M3) {
+        return e4m3_pair(x[0] * inv.lo, x[1] * inv.lo) | (e4m3_pair(x[2] * inv.lo, x[3] * inv.lo) << 16);
+    } else {
+        uint32_t b[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float t = fmaf(x[i], inv, kMagic);
-        off = fmaxf(off, fabsf(fmaf(-(t - kMagic), s, x[i])));
-        b[i] = __float_as_uint(t);
+        for (int i = 0; i < 4; ++i) {
+            b[i] = __float_as_uint(fmaf(x[i], inv.lo, kMagic));
+            split |= b[i] ^ __float_as_uint(fmaf(x[i], inv.hi, kMagic));
+        }
+        return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     }
-    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+// The nearest integer to x / s, ties to even, for finite |x / s| <= 127.5: the remainder of a candidate that is off by one at
+// most is exact in one fma.
+__device__ __forceinline__ uint32_t encode_near(float x, float s, float inv) {
+    float q = fmaf(x, inv, kMagic) - kMagic;
+    const float r = fmaf(-q, s, x), two = 2.f * fabsf(r);
+    if (two > s || (two == s && (static_cast<int>(q) & 1))) q += r > 0.f ? 1.f : -1.f;
+    return static_cast<uint32_t>(static_cast<int>(q)) & 0xffu;
 }
 
 // A code in a scale that has grown by 2^k; f = 2^-k.
@@ -163,172 +187,188 @@ __device__ __forceinline__ CopyUnit find_unit(const QuantCopyArgs& a, int u) {
     return un;
 }
 
-// A lane's 16 elements of a row: vectors of 16 bytes, LPR lanes apart, so that a load covers whole lines.
-template <typename T, int LPR>
-struct Row16 {
-    static constexpr int N = 16 / Vec16<T>::N;   // vectors
-    static constexpr int E = Vec16<T>::N;        // elements of one
-    uint4 v[N];
-    static __device__ __forceinline__ int col(int i, int cl) { return (i * LPR + cl) * E; }   // first element of vector i
-    __device__ __forceinline__ void load(const T* row, int cl, int D, bool in) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = in && col(i, cl) < D ? __ldg(reinterpret_cast<const uint4*>(row + col(i, cl))) : make_uint4(0, 0, 0, 0);
+// The bits of the largest magnitude of a 16-byte vector as fp32: above those of infinity if there is a NaN, equal if there is
+// an infinity.
+template <typename T>
+__device__ __forceinline__ uint32_t top_of(const uint4& v) {
+    if constexpr (sizeof(T) == 2) {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        const T2* w = reinterpret_cast<const T2*>(&v);
+        const T2 u = __hmax2_nan(__hmax2_nan(__habs2(w[0]), __habs2(w[1])), __hmax2_nan(__habs2(w[2]), __habs2(w[3])));
+        return __float_as_uint(Cvt<T>::to_f(__hmax_nan(u.x, u.y))) & 0x7fffffffu;
+    } else {
+        return max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
     }
-    // The bits of the largest magnitude as fp32: above those of infinity if there is a NaN, equal if there is an infinity.
-    __device__ __forceinline__ uint32_t top() const {
-        uint32_t m = 0;
-        if constexpr (sizeof(T) == 2) {
-            // magnitudes of a 16-bit float type are ordered as integers
-            uint32_t u = 0;
+}
+template <typename T>
+__device__ __forceinline__ float finite_top_of(const uint4& v) {
+    float f[Vec16<T>::N], m = 0.f;
+    unpack16<T>(v, f);
 #pragma unroll
-            for (int i = 0; i < N; ++i) u = __vmaxu2(__vmaxu2(u, __vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu)), __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
-            const uint32_t w = max(u & 0xffffu, u >> 16);
-            const unsigned short h = static_cast<unsigned short>(w);
-            m = __float_as_uint(Cvt<T>::to_f(*reinterpret_cast<const T*>(&h))) & 0x7fffffffu;
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                m = max(max(m, max(v[i].x & 0x7fffffffu, v[i].y & 0x7fffffffu)), max(v[i].z & 0x7fffffffu, v[i].w & 0x7fffffffu));
-        }
-        return m;
-    }
-    __device__ __forceinline__ float finite_top() const {
-        float m = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float f[E];
-            unpack16<T>(v[i], f);
-#pragma unroll
-            for (int j = 0; j < E; ++j) m = fmaxf(m, isfinite(f[j]) ? fabsf(f[j]) : 0.f);
-        }
-        return m;
-    }
-};
+    for (int j = 0; j < Vec16<T>::N; ++j) m = fmaxf(m, isfinite(f[j]) ? fabsf(f[j]) : 0.f);
+    return m;
+}
 
 constexpr uint32_t kInfBits = 0x7f800000u;
 
 // CTAs of an SM that the registers are to leave room for: the rows of a warp's 16 are held between the two passes.
 template <typename T>
-constexpr int copy_ctas(int lpr) { return sizeof(T) * lpr <= 16 ? 4 : sizeof(T) * lpr <= 32 ? 2 : 1; }
+constexpr int copy_ctas(int lpr) { return sizeof(T) * lpr <= 8 ? 4 : sizeof(T) * lpr <= 16 ? 3 : sizeof(T) * lpr <= 32 ? 2 : 1; }
 
-// Lanes of a row LPR (16 elements each; where the row is shorter some vectors are left out), W warps of 16 rows to a unit.
+// One row of a unit with a NaN or an infinity in it; the lanes of a row share it.
+template <typename T, bool E4M3>
+__device__ __noinline__ void encode_row_slow(const T* x, uint8_t* to, int D, int first, int step, float s) {
+    for (int d = first; d < D; d += step) to[d] = static_cast<uint8_t>(encode_slow<E4M3>(Cvt<T>::to_f(x[d]), s));
+}
+
+// What earlier calls left in a block, in a scale grown by 2^steps: rows p, p + by, ... below p0, 16 codes of each.
+template <bool E4M3>
+__device__ __noinline__ void shrink_rows(uint8_t* dst, int64_t pitch, int p, int p0, int by, int steps) {
+    const float f = pow2f(-steps);
+    for (; p < p0; p += by) {
+        uint4* at = reinterpret_cast<uint4*>(dst + static_cast<int64_t>(p) * pitch);
+        uint4 v = *at;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            uint32_t o = 0;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) o |= shrink_code((w[e] >> (8 * b)) & 0xffu, f, E4M3) << (8 * b);
+            w[e] = o;
+        }
+        *at = v;
+    }
+}
+
+// Lanes of a row LPR, with 16 elements each: vectors of 16 bytes, LPR lanes apart, so that a load covers whole lines (where the
+// row is shorter some vectors are left out). W warps of 16 rows to a unit.
 template <typename T, bool E4M3, int LPR, int W, bool REREAD>
 __global__ void __launch_bounds__(kCopyThreads, copy_ctas<T>(LPR)) quantized_copy_kernel(const QuantCopyArgs a) {
-    using Row = Row16<T, LPR>;
+    constexpr int E = Vec16<T>::N;             // elements of a vector
+    constexpr int N = 16 / E;                  // vectors of a lane's row
     constexpr int RPP = 32 / LPR;              // rows of a warp's pass
     constexpr int PASSES = kWarpRows / RPP;
     constexpr int UPC = kCopyWarps / W;        // heads of a CTA
     __shared__ uint32_t s_top[2][kCopyWarps];
-    const int m = blockIdx.z;                  // 0: K, 1: V
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const CopyUnit un = find_unit(a, blockIdx.x);
     if (un.block < 0) return;                  // the same for the whole CTA
     const int h = blockIdx.y * UPC + warp / W, wu = warp % W;
     const bool here = h < a.H;
     const int rl = lane / LPR, cl = lane % LPR;
-    const T* src = static_cast<const T*>(a.src[m]) + static_cast<int64_t>(h) * a.src_s1[m];
-    uint8_t* dst = static_cast<uint8_t*>(a.cache[m]) + un.block * a.c_s0[m] + static_cast<int64_t>(h) * a.c_s2[m];
-    float* scale = a.scale[m] + un.block * a.s_s0[m] + static_cast<int64_t>(h) * a.s_s1[m];
+    const bool full_width = a.D == 16 * LPR;
 
-    // Row of pass i of chunk q in the block. Only the rows of the call are loaded.
-    const int chunks = REREAD ? (un.p1 + W * kWarpRows - 1) / (W * kWarpRows) : 1;
-    auto row_of = [&](int q, int i) { return (q * W + wu) * kWarpRows + i * RPP + rl; };
-    Row r[PASSES];
-    auto load_rows = [&](int q) {
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int p = row_of(q, i);
-            const bool in = here && p >= un.p0 && p < un.p1;
-            r[i].load(src + (un.row0 + (in ? p - un.p0 : 0)) * a.src_s0[m], cl, a.D, in);
-        }
-    };
-    const float old = here && un.p0 > 0 ? *scale : 0.f;   // read by every lane before the barrier below, written after it
+    // K and V one after the other, or (two CTAs along z) one of them
+#pragma unroll 1
+    for (int m = blockIdx.z; m < 2; m += gridDim.z) {
+        const int64_t pitch = a.src_s0[m];
+        // row of position 0 of this block, in front of the first row when the call does not write it: not read there
+        const T* src = static_cast<const T*>(a.src[m]) + (un.row0 - un.p0) * pitch + static_cast<int64_t>(h) * a.src_s1[m];
+        uint8_t* dst = static_cast<uint8_t*>(a.cache[m]) + un.block * a.c_s0[m] + static_cast<int64_t>(h) * a.c_s2[m];
+        float* scale = a.scale[m] + un.block * a.s_s0[m] + static_cast<int64_t>(h) * a.s_s1[m];
 
-    uint32_t top = 0;
-    for (int q = 0; q < chunks; ++q) {
-        load_rows(q);
+        const int chunks = REREAD ? (un.p1 + W * kWarpRows - 1) / (W * kWarpRows) : 1;
+        uint4 r[PASSES][N];
+        // The rows of chunk q that belong to the call; a unit whose every row does, at full width, needs no looking.
+        auto load_rows = [&](int q) {
+            const int p = (q * W + wu) * kWarpRows + rl;
+            const T* from = src + p * pitch + cl * E;
+            const bool whole = full_width && here && p - rl >= un.p0 && p - rl + kWarpRows <= un.p1;
+            if (whole) {
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) top = max(top, r[i].top());
-    }
-    auto over_unit = [&](uint32_t x, int buf) {   // the largest of a unit
-        x = __reduce_max_sync(0xffffffffu, x);
-        if constexpr (W > 1) {
-            if (lane == 0) s_top[buf][warp] = x;
-            __syncthreads();
+                for (int i = 0; i < PASSES; ++i) {
 #pragma unroll
-            for (int w = 0; w < W; ++w) x = max(x, s_top[buf][warp / W * W + w]);
+                    for (int n = 0; n < N; ++n) r[i][n] = __ldg(reinterpret_cast<const uint4*>(from + n * LPR * E));
+                    from += RPP * pitch;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < PASSES; ++i) {
+                    const bool in = here && p + i * RPP >= un.p0 && p + i * RPP < un.p1;
+#pragma unroll
+                    for (int n = 0; n < N; ++n)
+                        r[i][n] = in && (n * LPR + cl) * E < a.D ? __ldg(reinterpret_cast<const uint4*>(from + n * LPR * E)) : make_uint4(0, 0, 0, 0);
+                    from += RPP * pitch;
+                }
+            }
+        };
+        const float old = here && un.p0 > 0 ? *scale : 0.f;   // read by every lane before the barrier below, written after it
+
+        uint32_t top = 0;
+        for (int q = 0; q < chunks; ++q) {
+            load_rows(q);
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+                for (int n = 0; n < N; ++n) top = max(top, top_of<T>(r[i][n]));
         }
-        return x;
-    };
-    top = over_unit(top, 0);
-    const bool odd = top >= kInfBits;   // a NaN or an infinity in the unit: it does not count
-    if (W > 1 ? __syncthreads_or(odd) != 0 : odd) {
-        uint32_t f = 0;
+        auto over_unit = [&](uint32_t x, int buf) {   // the largest of a unit
+            x = __reduce_max_sync(0xffffffffu, x);
+            if constexpr (W > 1) {
+                if (lane == 0) s_top[buf][warp] = x;
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < W; ++w) x = max(x, s_top[buf][warp / W * W + w]);
+            }
+            return x;
+        };
+        top = over_unit(top, 0);
+        const bool odd = top >= kInfBits;   // a NaN or an infinity in the unit: it does not count
+        if (W > 1 ? __syncthreads_or(odd) != 0 : odd) {
+            uint32_t f = 0;
+            for (int q = 0; q < chunks; ++q) {
+                if (REREAD) load_rows(q);
+#pragma unroll
+                for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+                    for (int n = 0; n < N; ++n) f = max(f, __float_as_uint(finite_top_of<T>(r[i][n])));
+            }
+            top = over_unit(f, 1);
+        }
+
+        float s = fresh_scale(__uint_as_float(top), E4M3);
+        if (here && un.p0 > 0 && old > 0.f) {
+            const int steps = growth_steps(old, s);
+            s = steps > 0 ? static_cast<float>(scalbn(static_cast<double>(old), steps)) : old;
+            if (steps > 0 && cl * 16 < a.D) shrink_rows<E4M3>(dst + cl * 16, a.c_s1[m], wu * RPP + rl, un.p0, W * RPP, steps);
+        }
+        if (here && wu == 0 && lane == 0) *scale = s;
+
+        const Inverse inv = inverse_of<E4M3>(s);
         for (int q = 0; q < chunks; ++q) {
             if (REREAD) load_rows(q);
+            const int p = (q * W + wu) * kWarpRows + rl;
+            uint8_t* to = dst + p * a.c_s1[m] + cl * E;
 #pragma unroll
-            for (int i = 0; i < PASSES; ++i) f = max(f, __float_as_uint(r[i].finite_top()));
-        }
-        top = over_unit(f, 1);
-    }
-    if (!here) return;
-
-    float s = fresh_scale(__uint_as_float(top), E4M3);
-    if (un.p0 > 0 && old > 0.f) {
-        const int steps = growth_steps(old, s);
-        s = steps > 0 ? static_cast<float>(scalbn(static_cast<double>(old), steps)) : old;
-        if (steps > 0) {   // what earlier calls left in this block, in the grown scale
-            const float f = pow2f(-steps);
-            for (int p = wu * kWarpRows + rl; p < un.p0; p += (p % kWarpRows + RPP < kWarpRows) ? RPP : (W - 1) * kWarpRows + RPP) {
-                if (cl * 16 >= a.D) continue;
-                uint4* at = reinterpret_cast<uint4*>(dst + static_cast<int64_t>(p) * a.c_s1[m] + cl * 16);
-                uint4 v = *at;
-                uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+            for (int i = 0; i < PASSES; ++i) {
+                const bool in = here && p + i * RPP >= un.p0 && p + i * RPP < un.p1;
+                if (in && odd) {
+                    encode_row_slow<T, E4M3>(src + (p + i * RPP) * pitch, to - cl * E, a.D, cl, LPR, s);
+                } else if (in) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    uint32_t o = 0;
+                    for (int n = 0; n < N; ++n) {
+                        if (!full_width && (n * LPR + cl) * E >= a.D) continue;
+                        float f[E];
+                        unpack16<T>(r[i][n], f);
+                        uint32_t w[E / 4], split = 0;
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) o |= shrink_code((w[e] >> (8 * b)) & 0xffu, f, E4M3) << (8 * b);
-                    w[e] = o;
-                }
-                *at = v;
-            }
-        }
-    }
-    if (wu == 0 && lane == 0) *scale = s;
-
-    const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
-    const float half_step = s > 0.f ? 0.5f * s : INFINITY;
-    for (int q = 0; q < chunks; ++q) {
-        if (REREAD) load_rows(q);
+                        for (int e = 0; e < E / 4; ++e) w[e] = encode4<E4M3>(f + 4 * e, inv, split);
+                        if (!E4M3 && split != 0) {
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int p = row_of(q, i);
-            if (p < un.p0 || p >= un.p1) continue;
-            uint8_t* row = dst + static_cast<int64_t>(p) * a.c_s1[m];
-#pragma unroll
-            for (int n = 0; n < Row::N; ++n) {
-                if (Row::col(n, cl) >= a.D) continue;
-                float f[Row::E];
-                unpack16<T>(r[i].v[n], f);
-                uint32_t w[Row::E / 4];
-                float off = 0.f;
-#pragma unroll
-                for (int e = 0; e < Row::E / 4; ++e) w[e] = encode4<E4M3>(f + 4 * e, s, inv, off);
-                if (odd || (!E4M3 && off >= half_step)) {
-#pragma unroll
-                    for (int e = 0; e < Row::E / 4; ++e) {
-                        w[e] = 0;
-#pragma unroll
-                        for (int b = 0; b < 4; ++b) w[e] |= encode_slow<E4M3>(f[4 * e + b], s) << (8 * b);
+                            for (int e = 0; e < E / 4; ++e)
+                                w[e] = encode_near(f[4 * e], s, inv.lo) | (encode_near(f[4 * e + 1], s, inv.lo) << 8) | (encode_near(f[4 * e + 2], s, inv.lo) << 16) |
+                                       (encode_near(f[4 * e + 3], s, inv.lo) << 24);
+                        }
+                        if constexpr (E == 8)
+                            *reinterpret_cast<uint2*>(to + n * LPR * E) = make_uint2(w[0], w[1]);
+                        else
+                            *reinterpret_cast<uint32_t*>(to + n * LPR * E) = w[0];
                     }
                 }
-                if constexpr (Row::E == 8)
-                    *reinterpret_cast<uint2*>(row + Row::col(n, cl)) = make_uint2(w[0], w[1]);
-                else
-                    *reinterpret_cast<uint32_t*>(row + Row::col(n, cl)) = w[0];
+                to += RPP * a.c_s1[m];
             }
         }
+        if constexpr (W > 1) __syncthreads();   // s_top is written again
     }
 }
 
@@ -374,10 +414,12 @@ __global__ void __launch_bounds__(kCopyThreads) quantized_copy_any_kernel(const 
 }
 
 template <typename T, bool E4M3, int LPR>
-void launch_rows(const QuantCopyArgs& a, int units, cudaStream_t st) {
+void launch_rows(const QuantCopyArgs& a, int units, int sm_count, cudaStream_t st) {
     auto go = [&](auto kern, int w) {
         const int upc = kCopyWarps / w;
-        kern<<<dim3(units, (a.H + upc - 1) / upc, 2), kCopyThreads, 0, st>>>(a);
+        const int y = (a.H + upc - 1) / upc;
+        // Few CTAs: K and V side by side (64 requests of one token: 6.2 us; 8.0 one after the other); many: one look-up for both.
+        kern<<<dim3(units, y, static_cast<int64_t>(units) * y < 8 * sm_count ? 2 : 1), kCopyThreads, 0, st>>>(a);
     };
     if (a.block_size <= 16) go(quantized_copy_kernel<T, E4M3, LPR, 1, false>, 1);
     else if (a.block_size <= 32) go(quantized_copy_kernel<T, E4M3, LPR, 2, false>, 2);
@@ -387,12 +429,12 @@ void launch_rows(const QuantCopyArgs& a, int units, cudaStream_t st) {
 }
 
 template <typename T, int LPR>
-void launch_kind(const QuantCopyArgs& a, int units, cudaStream_t st) {
-    a.e4m3 ? launch_rows<T, true, LPR>(a, units, st) : launch_rows<T, false, LPR>(a, units, st);
+void launch_kind(const QuantCopyArgs& a, int units, int sm_count, cudaStream_t st) {
+    a.e4m3 ? launch_rows<T, true, LPR>(a, units, sm_count, st) : launch_rows<T, false, LPR>(a, units, sm_count, st);
 }
 
 template <typename T>
-void launch_t(const QuantCopyArgs& a, int units, cudaStream_t st) {
+void launch_t(const QuantCopyArgs& a, int units, int sm_count, cudaStream_t st) {
     bool rows = a.D % 16 == 0 && a.D <= 256;
     for (int m = 0; m < 2; ++m) {
         rows = rows && a.src_s2[m] == 1 && (a.src_s0[m] * sizeof(T)) % 16 == 0 && (a.src_s1[m] * sizeof(T)) % 16 == 0 &&
@@ -403,25 +445,25 @@ void launch_t(const QuantCopyArgs& a, int units, cudaStream_t st) {
     if (!rows)
         quantized_copy_any_kernel<T><<<dim3(units, a.H, 2), kCopyThreads, 0, st>>>(a);
     else if (a.D <= 64)
-        launch_kind<T, 4>(a, units, st);
+        launch_kind<T, 4>(a, units, sm_count, st);
     else if (a.D <= 128)
-        launch_kind<T, 8>(a, units, st);
+        launch_kind<T, 8>(a, units, sm_count, st);
     else
-        launch_kind<T, 16>(a, units, st);
+        launch_kind<T, 16>(a, units, sm_count, st);
 }
 
 }  // namespace
 
-void launch_quantized_copy_kv(const QuantCopyArgs& a, cudaStream_t st) {
+void launch_quantized_copy_kv(const QuantCopyArgs& a, int sm_count, cudaStream_t st) {
     // Touched blocks of a request of n tokens: n at most, and n / block_size + 2 at most.
     const int64_t units = std::min<int64_t>(a.T, a.T / a.block_size + 2ll * a.B);
     if (units <= 0) return;
     if (a.dt == Dt::F16)
-        launch_t<__half>(a, static_cast<int>(units), st);
+        launch_t<__half>(a, static_cast<int>(units), sm_count, st);
     else if (a.dt == Dt::BF16)
-        launch_t<__nv_bfloat16>(a, static_cast<int>(units), st);
+        launch_t<__nv_bfloat16>(a, static_cast<int>(units), sm_count, st);
     else
-        launch_t<float>(a, static_cast<int>(units), st);
+        launch_t<float>(a, static_cast<int>(units), sm_count, st);
 }
 
 }  // namespace k

@@ -1,0 +1,181 @@
+// One call of an exported op from Python without the interpreter's work in between: takes the torch tensors of the call,
+// makes their handles through the run time beside it, calls the op and frees the handles. It reads tensors through their
+// Python attributes (shape, stride(), data_ptr(), dtype, is_cuda), so nothing of torch is needed to build or load it.
+// Through ctypes the same call spends three times as long in Python as in the op: 15 us against 5 for ten tensors.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <cstdint>
+#include <utility>
+
+namespace {
+
+constexpr int kMaxTensors = 12;
+constexpr int kMaxNdim = 16;
+
+using BatchCreate = void* (*)(const int64_t*, int, void**);
+using BatchDestroy = void (*)(void*);
+
+struct State {
+    BatchCreate create = nullptr;
+    BatchDestroy destroy = nullptr;
+    PyObject* dtypes = nullptr;        // torch dtype -> diopiDtype_t
+    PyTypeObject* handle = nullptr;    // the class whose `handle` attribute is a tensor handle already
+    PyObject *shape = nullptr, *stride = nullptr, *data_ptr = nullptr, *dtype = nullptr, *is_cuda = nullptr, *handle_name = nullptr;
+} g;
+
+struct Ref {   // owns one reference
+    PyObject* p;
+    explicit Ref(PyObject* o) : p(o) {}
+    Ref(const Ref&) = delete;
+    ~Ref() { Py_XDECREF(p); }
+};
+
+bool put_tuple(PyObject* t, Py_ssize_t n, int64_t*& d) {
+    if (!PyTuple_Check(t) || PyTuple_GET_SIZE(t) != n) {
+        PyErr_SetString(PyExc_TypeError, "a tensor's shape and stride() must be tuples of its number of dims");
+        return false;
+    }
+    for (Py_ssize_t i = 0; i < n; ++i) *d++ = PyLong_AsLongLong(PyTuple_GET_ITEM(t, i));
+    return !PyErr_Occurred();
+}
+
+// Appends one tensor's description; `as_device` < 0: where it says it is.
+bool describe(PyObject* t, int as_device, int64_t*& d) {
+    Ref dt(PyObject_GetAttr(t, g.dtype));
+    if (!dt.p) return false;
+    PyObject* code = PyDict_GetItemWithError(g.dtypes, dt.p);
+    if (!code) {
+        if (!PyErr_Occurred()) PyErr_Format(PyExc_TypeError, "dtype %S has no DIOPI counterpart", dt.p);
+        return false;
+    }
+    Ref shape(PyObject_GetAttr(t, g.shape));
+    if (!shape.p) return false;
+    const Py_ssize_t nd = PyTuple_Check(shape.p) ? PyTuple_GET_SIZE(shape.p) : -1;
+    if (nd > kMaxNdim) {
+        PyErr_Format(PyExc_ValueError, "a tensor has %zd dims; at most %d are supported", nd, kMaxNdim);
+        return false;
+    }
+    Ref stride(PyObject_CallMethodNoArgs(t, g.stride));
+    if (!stride.p) return false;
+    Ref ptr(PyObject_CallMethodNoArgs(t, g.data_ptr));
+    if (!ptr.p) return false;
+    if (as_device < 0) {
+        Ref cuda(PyObject_GetAttr(t, g.is_cuda));
+        if (!cuda.p) return false;
+        as_device = cuda.p == Py_True;
+    }
+    *d++ = nd;
+    *d++ = PyLong_AsLongLong(code);
+    *d++ = as_device;
+    *d++ = static_cast<int64_t>(PyLong_AsUnsignedLongLong(ptr.p));
+    return put_tuple(shape.p, nd, d) && put_tuple(stride.p, nd, d);
+}
+
+template <typename... Extra, size_t... I>
+int call_n(void* fn, void* ctx, void** h, std::index_sequence<I...>, Extra... extra) {
+    return reinterpret_cast<int (*)(void*, decltype(static_cast<void>(I), static_cast<void*>(nullptr))..., Extra...)>(fn)(ctx, h[I]..., extra...);
+}
+template <typename... Extra>
+int call_op(void* fn, void* ctx, void** h, Py_ssize_t n, Extra... extra) {
+    switch (n) {
+        case 8: return call_n(fn, ctx, h, std::make_index_sequence<8>{}, extra...);
+        case 9: return call_n(fn, ctx, h, std::make_index_sequence<9>{}, extra...);
+        case 10: return call_n(fn, ctx, h, std::make_index_sequence<10>{}, extra...);
+        default: return -1;
+    }
+}
+
+// call(op address, context handle, tuple of tensors, extra argument or None, as_device or None) -> return code. The op
+// takes the context, the tensors' handles and then the extra argument (an int as int64_t, a float as double).
+PyObject* call(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    if (na != 5 || !PyTuple_Check(a[2]) || !g.create) {
+        PyErr_SetString(PyExc_TypeError, "call(op, context, tensors, extra, as_device) after init()");
+        return nullptr;
+    }
+    void* fn = PyLong_AsVoidPtr(a[0]);
+    void* ctx = PyLong_AsVoidPtr(a[1]);
+    if (PyErr_Occurred()) return nullptr;
+    const Py_ssize_t n = PyTuple_GET_SIZE(a[2]);
+    if (n < 8 || n > 10) {
+        PyErr_SetString(PyExc_TypeError, "ops of 8 to 10 tensors are called this way");
+        return nullptr;
+    }
+    const int as_device = a[4] == Py_None ? -1 : PyObject_IsTrue(a[4]);
+    int64_t desc[kMaxTensors * (4 + 2 * kMaxNdim)];
+    void* given[kMaxTensors] = {nullptr};
+    int64_t* d = desc;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject* t = PyTuple_GET_ITEM(a[2], i);
+        if (t == Py_None) {
+            *d++ = -1;
+        } else if (Py_TYPE(t) == g.handle) {
+            Ref h(PyObject_GetAttr(t, g.handle_name));
+            if (!h.p) return nullptr;
+            given[i] = PyLong_AsVoidPtr(h.p);
+            if (PyErr_Occurred()) return nullptr;
+            *d++ = -1;
+        } else if (!describe(t, as_device, d) || PyErr_Occurred()) {
+            return nullptr;
+        }
+    }
+    int64_t whole = 0;
+    double real = 0;
+    const bool is_real = PyFloat_Check(a[3]);
+    if (is_real)
+        real = PyFloat_AS_DOUBLE(a[3]);
+    else if (a[3] != Py_None)
+        whole = PyLong_AsLongLong(a[3]);
+    if (PyErr_Occurred()) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS;
+    void* h[kMaxTensors];
+    void* batch = g.create(desc, static_cast<int>(n), h);
+    for (Py_ssize_t i = 0; i < n; ++i)
+        if (given[i]) h[i] = given[i];
+    if (is_real)
+        rc = call_op(fn, ctx, h, n, real);
+    else if (a[3] != Py_None)
+        rc = call_op(fn, ctx, h, n, whole);
+    else
+        rc = call_op(fn, ctx, h, n);
+    g.destroy(batch);
+    Py_END_ALLOW_THREADS;
+    return PyLong_FromLong(rc);
+}
+
+// init(address of b200rt_batch_create, address of b200rt_batch_destroy, dict of dtypes, handle class)
+PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    if (na != 4 || !PyDict_Check(a[2]) || !PyType_Check(a[3])) {
+        PyErr_SetString(PyExc_TypeError, "init(create, destroy, dtypes, handle class)");
+        return nullptr;
+    }
+    g.create = reinterpret_cast<BatchCreate>(PyLong_AsVoidPtr(a[0]));
+    g.destroy = reinterpret_cast<BatchDestroy>(PyLong_AsVoidPtr(a[1]));
+    if (PyErr_Occurred()) return nullptr;
+    Py_INCREF(a[2]);
+    Py_XSETREF(g.dtypes, a[2]);
+    Py_INCREF(a[3]);
+    Py_XDECREF(reinterpret_cast<PyObject*>(g.handle));
+    g.handle = reinterpret_cast<PyTypeObject*>(a[3]);
+    Py_RETURN_NONE;
+}
+
+PyMethodDef methods[] = {
+    {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call)), METH_FASTCALL, nullptr},
+    {"init", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(init)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr},
+};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit__pycall() {
+    g.shape = PyUnicode_InternFromString("shape");
+    g.stride = PyUnicode_InternFromString("stride");
+    g.data_ptr = PyUnicode_InternFromString("data_ptr");
+    g.dtype = PyUnicode_InternFromString("dtype");
+    g.is_cuda = PyUnicode_InternFromString("is_cuda");
+    g.handle_name = PyUnicode_InternFromString("handle");
+    return PyModule_Create(&module);
+}

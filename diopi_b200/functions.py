@@ -32,10 +32,9 @@ def _call(name: str, ctx: Context | None, *args):
     check_returncode(name, rc)
 
 
-def _run(name: str, ctx: Context | None, tensors, as_device, *args):
+def _run(name: str, ctx: Context | None, tensors: tuple, as_device, extra=None):
     """One call whose handles live as long as it does."""
-    ctx = ctx or default_context()
-    rc = call_with(getattr(_impl(), name), ctx.handle, tensors, args, as_device)
+    rc = call_with(name, (ctx or default_context()).handle, tensors, extra, as_device)
     if rc:
         check_returncode(name, rc)
 

@@ -8,7 +8,6 @@ a kernel) is handed to the C ABI by pointer, shape and stride, without a copy.
 from __future__ import annotations
 
 import ctypes
-from array import array
 from ctypes import c_int64
 
 import torch
@@ -76,38 +75,19 @@ class Tensor:
             self._rt.b200rt_tensor_destroy(h)
 
 
-def call_with(fn, ctx_handle, tensors, args, as_device: bool | None = None) -> int:
-    """fn(ctx, handles of `tensors`, *args) with handles that live as long as the call. Each item is a torch tensor, a
-    Tensor or None. Cheaper than one Tensor each: one call into the run time for all of them."""
-    rt = _lib.load().rt
-    desc = []
-    given = None
-    for i, t in enumerate(tensors):
-        if t is None:
-            desc.append(-1)
-        elif isinstance(t, Tensor):
-            desc.append(-1)
-            given = given or []
-            given.append((i, t.handle))
-        else:
-            code = _TORCH_TO_DIOPI.get(t.dtype)
-            if code is None:
-                raise TypeError(f"dtype {t.dtype} has no DIOPI counterpart")
-            shape = t.shape
-            desc += (len(shape), code, t.is_cuda if as_device is None else as_device, t.data_ptr())
-            desc += shape
-            desc += t.stride()
-    n = len(tensors)
-    packed = array("q", desc)
-    out = array("Q", bytes(8 * n))
-    batch = rt.b200rt_batch_create(packed.buffer_info()[0], n, out.buffer_info()[0])
-    try:
-        if given:
-            for i, h in given:
-                out[i] = h
-        return fn(ctx_handle, *[h or None for h in out], *args)
-    finally:
-        rt.b200rt_batch_destroy(batch)
+_pycall = None
+
+
+def call_with(op: str, ctx_handle, tensors: tuple, extra=None, as_device: bool | None = None) -> int:
+    """The return code of op(ctx, handles of `tensors`..., extra), with handles that live as long as the call. Each item is
+    a torch tensor, a Tensor or None; `extra` an int (int64_t), a float (double) or None."""
+    global _pycall
+    if _pycall is None:
+        libs = _lib.load()
+        address = lambda fn: ctypes.cast(fn, ctypes.c_void_p).value  # noqa: E731
+        libs.pycall.init(address(libs.rt.b200rt_batch_create), address(libs.rt.b200rt_batch_destroy), _TORCH_TO_DIOPI, Tensor)
+        _pycall = libs.pycall.call
+    return _pycall(_lib._libs.address[op], ctx_handle, tensors, extra, as_device)
 
 
 class Context:
