@@ -80,6 +80,8 @@ struct BlockTableArgs {
     int B, cols, block_size;
     int64_t T, wide_cols, n_free;
     int* status;
+    uint32_t div_mul;          // set by the launch: division by block_size as a product and a shift
+    int div_shift;
 };
 void launch_block_table(const BlockTableArgs& a, int sm_count, cudaStream_t st);
 
