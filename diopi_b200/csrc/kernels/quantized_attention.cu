@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
     __syncthreads();
 
     const int team = warp / p.mt, mtile = warp - team * p.mt;
-    const int hl = team % p.hw, range = blockIdx.x * p.tw + team / p.hw;
+    const int hl = team % p.hw, range = team / p.hw * p.n_cta + blockIdx.x;   // few ranges: spread over the SMs
     const int total = pre[a.B];
     const int used = used_ranges(total, p.n_range);
     if (team < teams && range < used && total > 0) {
@@ -460,9 +460,9 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
             if (valid > 0) {
                 const uint32_t kt = ring0 + slot * STAGE;
                 // ---- S^T = Kc Q^T: 16 tokens by 8 query rows ----
-                float s[NT][4];
+                float s[NT][4], s2[NT][4];   // every other k step: two chains of products side by side
 #pragma unroll
-                for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+                for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.f;
 #pragma unroll
                 for (int i = 0; i < CH; i += 4) {
                     const int cc = (i % (RB / 16)) + (lane >> 3);
@@ -477,10 +477,15 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                         codes_to_f16<E4M3>(d[m], f[1], f[3]);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            mma_f16(s[n], f, qf[n][i + m][0], qf[n][i + m][1]);
-                            if constexpr (SPLIT) mma_f16(s[n], f, ql[n][i + m][0], ql[n][i + m][1]);
+                            float (&to)[4] = NT == 1 && (m & 1) ? s2[n] : s[n];
+                            mma_f16(to, f, qf[n][i + m][0], qf[n][i + m][1]);
+                            if constexpr (SPLIT) mma_f16(to, f, ql[n][i + m][0], ql[n][i + m][1]);
                         }
                     }
+                }
+                if constexpr (NT == 1) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[0][e] += s2[0][e];
                 }
                 // ---- the codes of V, on their way while the weights are made ----
                 uint32_t v[NH][4][VB / 4];   // tokens 2c, 2c + 1, 2c + 8, 2c + 9
@@ -684,11 +689,12 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
 // read one after the other (four requests of 30011 to 131072 tokens: 145 us with one warp to a row, 5 us with eight).
 constexpr int kMergeWarps = 8;
 
-template <typename T, bool WIDE>   // WIDE: head_dim above 128
-__global__ void __launch_bounds__(32 * kMergeWarps, WIDE ? 3 : 4) quant_combine_kernel(const QuantAttnArgs a, int n_range, int wpr, const float* __restrict__ ws_acc,
+template <typename T, int HD>   // head_dim rounded up to 64 (two parts of a row side by side in a warp), 128 or 256
+__global__ void __launch_bounds__(32 * kMergeWarps, HD > 128 ? 3 : 4) quant_combine_kernel(const QuantAttnArgs a, int n_range, int wpr, const float* __restrict__ ws_acc,
                                                                          const float* __restrict__ ws_ml) {
     __shared__ int s_part[kMergeWarps][2];
-    constexpr int NV = WIDE ? 8 : 4;
+    constexpr bool WIDE = HD > 128;
+    constexpr int NV = WIDE ? 8 : 4, SIDE = HD == 64 ? 2 : 1, LANES = 32 / SIDE;
     __shared__ float s_acc[kMergeWarps][32 * NV + 1];
     const int i = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int before = 0, all = 0;
@@ -732,7 +738,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps, WIDE ? 3 : 4) quant_combine_
     const int64_t rows = static_cast<int64_t>(a.n) * a.Hq;
     const float* ml = ws_ml + ((static_cast<int64_t>(c_first) + i) * rows + row) * 2;
     const float* acc = ws_acc + ((static_cast<int64_t>(c_first) + i) * rows + row) * a.D;
-    float v[NV];   // d = 4 * lane .. + 3, and 128 further
+    const int dl = 4 * (lane % LANES);
+    float v[NV];   // d = dl .. + 3, and 128 further
 #pragma unroll
     for (int e = 0; e < NV; ++e) v[e] = 0.f;
     float L = 0.f;
@@ -741,17 +748,18 @@ __global__ void __launch_bounds__(32 * kMergeWarps, WIDE ? 3 : 4) quant_combine_
         for (int c = lane; c < parts; c += 32) M = fmaxf(M, ml[c * rows * 2]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        const bool d0 = 4 * lane < a.D, d1 = 4 * lane + 128 < a.D;
-        for (int c = sub; c < parts; c += 4 * wpr) {
+        const bool d0 = dl < a.D, d1 = dl + 128 < a.D;
+        const int by = wpr * SIDE;
+        for (int c = sub * SIDE + lane / LANES; c < parts; c += 4 * by) {
             float2 x[4];
             float4 y[4], z[WIDE ? 4 : 1];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const int64_t at = (c + u * wpr) * rows;
-                const bool in = c + u * wpr < parts;
+                const int64_t at = (c + u * by) * rows;
+                const bool in = c + u * by < parts;
                 x[u] = in ? *reinterpret_cast<const float2*>(ml + at * 2) : make_float2(-INFINITY, 0.f);
-                y[u] = in && d0 ? *reinterpret_cast<const float4*>(acc + at * a.D + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-                if constexpr (WIDE) z[u] = in && d1 ? *reinterpret_cast<const float4*>(acc + at * a.D + 4 * lane + 128) : make_float4(0.f, 0.f, 0.f, 0.f);
+                y[u] = in && d0 ? *reinterpret_cast<const float4*>(acc + at * a.D + dl) : make_float4(0.f, 0.f, 0.f, 0.f);
+                if constexpr (WIDE) z[u] = in && d1 ? *reinterpret_cast<const float4*>(acc + at * a.D + dl + 128) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -769,6 +777,11 @@ __global__ void __launch_bounds__(32 * kMergeWarps, WIDE ? 3 : 4) quant_combine_
                 }
             }
         }
+    }
+    if constexpr (SIDE == 2) {
+        L += __shfl_xor_sync(0xffffffffu, L, 16);
+#pragma unroll
+        for (int e = 0; e < NV; ++e) v[e] += __shfl_xor_sync(0xffffffffu, v[e], 16);
     }
     if (wpr > 1) {
 #pragma unroll
@@ -788,8 +801,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps, WIDE ? 3 : 4) quant_combine_
     T* out = static_cast<T*>(a.out) + static_cast<int64_t>(i) * a.o_s0 + static_cast<int64_t>(t) * a.o_s1 + static_cast<int64_t>(h) * a.o_s2;
 #pragma unroll
     for (int e = 0; e < NV; ++e) {
-        const int d = 4 * lane + (e & 3) + (e >> 2) * 128;
-        if (d < a.D) out[d] = Cvt<T>::from_f(v[e] * inv);
+        const int d = dl + (e & 3) + (e >> 2) * 128;
+        if (d < a.D && lane < LANES) out[d] = Cvt<T>::from_f(v[e] * inv);
     }
 }
 
@@ -898,7 +911,7 @@ void launch_split(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap&
     }
     kern<<<dim3(p.n_cta, p.n_hg, p.n_z), threads, p.smem_bytes, st>>>(a, p, mk, mv, acc, ml);
     int wpr = 1;
-    while (wpr < kMergeWarps && wpr * 8 * a.B < p.n_range) wpr *= 2;   // eight parts to a warp on average
+    while (wpr < kMergeWarps && wpr * (HD == 64 ? 16 : 8) * a.B < p.n_range) wpr *= 2;   // eight parts to a warp on average
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.B, (a.n * a.Hq + kMergeWarps / wpr - 1) / (kMergeWarps / wpr), 1);
     cfg.blockDim = dim3(32 * kMergeWarps);
@@ -908,7 +921,7 @@ void launch_split(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap&
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, HD > 128 ? quant_combine_kernel<T, true> : quant_combine_kernel<T, false>, a, p.n_range, wpr, static_cast<const float*>(acc), static_cast<const float*>(ml));
+    cudaLaunchKernelEx(&cfg, quant_combine_kernel<T, HD>, a, p.n_range, wpr, static_cast<const float*>(acc), static_cast<const float*>(ml));
 }
 
 template <typename T>
