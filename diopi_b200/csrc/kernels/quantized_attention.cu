@@ -689,8 +689,9 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
 // read one after the other (four requests of 30011 to 131072 tokens: 145 us with one warp to a row, 5 us with eight).
 constexpr int kMergeWarps = 8;
 
-template <typename T, int HD>   // head_dim rounded up to 64 (two parts of a row side by side in a warp), 128 or 256
-__global__ void __launch_bounds__(32 * kMergeWarps, HD > 128 ? 3 : 4) quant_combine_kernel(const QuantAttnArgs a, int n_range, int wpr, const float* __restrict__ ws_acc,
+// HD: head_dim rounded up to 64 (two parts of a row side by side in a warp), 128 or 256. U: parts that a warp asks for at once.
+template <typename T, int HD, int U>
+__global__ void __launch_bounds__(32 * kMergeWarps, U > 4 ? 1 : HD > 128 ? 3 : 4) quant_combine_kernel(const QuantAttnArgs a, int n_range, int wpr, const float* __restrict__ ws_acc,
                                                                          const float* __restrict__ ws_ml) {
     __shared__ int s_part[kMergeWarps][2];
     constexpr bool WIDE = HD > 128;
@@ -730,9 +731,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps, HD > 128 ? 3 : 4) quant_comb
         };
         c_first = range_of(before);
         parts = range_of(before + tiles - 1) - c_first + 1;
-        if (parts == 1) return;   // written by that range
     }
+    // Also where there is nothing to merge: this grid must not be done before the one that it depends on.
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (parts == 1) return;   // written by that range
     const int row = blockIdx.y * (kMergeWarps / wpr) + warp / wpr, sub = warp % wpr;
     const bool here = row < a.n * a.Hq;
     const int64_t rows = static_cast<int64_t>(a.n) * a.Hq;
@@ -750,11 +752,11 @@ __global__ void __launch_bounds__(32 * kMergeWarps, HD > 128 ? 3 : 4) quant_comb
         for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
         const bool d0 = dl < a.D, d1 = dl + 128 < a.D;
         const int by = wpr * SIDE;
-        for (int c = sub * SIDE + lane / LANES; c < parts; c += 4 * by) {
-            float2 x[4];
-            float4 y[4], z[WIDE ? 4 : 1];
+        for (int c = sub * SIDE + lane / LANES; c < parts; c += U * by) {
+            float2 x[U];
+            float4 y[U], z[WIDE ? U : 1];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < U; ++u) {
                 const int64_t at = (c + u * by) * rows;
                 const bool in = c + u * by < parts;
                 x[u] = in ? *reinterpret_cast<const float2*>(ml + at * 2) : make_float2(-INFINITY, 0.f);
@@ -762,7 +764,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps, HD > 128 ? 3 : 4) quant_comb
                 if constexpr (WIDE) z[u] = in && d1 ? *reinterpret_cast<const float4*>(acc + at * a.D + dl + 128) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < U; ++u) {
                 const float w = exp2f(x[u].x - M);
                 L = fmaf(x[u].y, w, L);
                 v[0] = fmaf(y[u].x, w, v[0]);
@@ -921,7 +923,7 @@ void launch_split(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap&
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, quant_combine_kernel<T, HD>, a, p.n_range, wpr, static_cast<const float*>(acc), static_cast<const float*>(ml));
+    cudaLaunchKernelEx(&cfg, wpr == kMergeWarps ? quant_combine_kernel<T, HD, 8> : quant_combine_kernel<T, HD, 4>, a, p.n_range, wpr, static_cast<const float*>(acc), static_cast<const float*>(ml));
 }
 
 template <typename T>

@@ -80,14 +80,16 @@ _pycall = None
 
 def call_with(op: str, ctx_handle, tensors: tuple, extra=None, as_device: bool | None = None) -> int:
     """The return code of op(ctx, handles of `tensors`..., extra), with handles that live as long as the call. Each item is
-    a torch tensor, a Tensor or None; `extra` an int (int64_t), a float (double) or None."""
+    a torch tensor, a Tensor or None; `extra` an int (int64_t), a float (double) or None. Tensors of another device than
+    the current one are refused: the op would be launched beside its own memory."""
     global _pycall
     if _pycall is None:
         libs = _lib.load()
         address = lambda fn: ctypes.cast(fn, ctypes.c_void_p).value  # noqa: E731
         libs.pycall.init(address(libs.rt.b200rt_batch_create), address(libs.rt.b200rt_batch_destroy), _TORCH_TO_DIOPI, Tensor)
         _pycall = libs.pycall.call
-    return _pycall(_lib._libs.address[op], ctx_handle, tensors, extra, as_device)
+    current = torch.cuda.current_device() if as_device is None and torch.cuda.is_initialized() else -1
+    return _pycall(_lib._libs.address[op], ctx_handle, tensors, extra, as_device, current)
 
 
 class Context:
