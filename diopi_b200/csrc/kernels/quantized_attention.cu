@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(32 * kPlainWarps) quant_plain_kernel(const Qua
 constexpr int kQMaxStages = 8;
 constexpr int kQMaxB = 4096;
 constexpr int kTile = 16;                       // tokens of a tile
-constexpr int kTilesPerRange = 4;               // at least, so that short batches are not cut into crumbs
+constexpr int kTilesPerRange = 4;               // at least, so that short batches are not cut into crumbs (2: the same times, twice the parts)
 
 // Warps of a CTA: as many as the registers of a thread's queries and accumulators leave room for (a spilled register costs
 // an L2 access here, as shared memory leaves no L1).
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                     float f0 = ks * rs[n][0], f1 = ks * rs[n][1];
                     if (!whole) {
                         const int r = rbase + 8 * n + 2 * c;
-                        const int n0 = min(valid, lim_min + r / group - pos), n1 = min(valid, lim_min + (r + 1) / group - pos);
+                        const int n0 = min(valid, lim_min + (a.n > 1 ? r / group : 0) - pos), n1 = min(valid, lim_min + (a.n > 1 ? (r + 1) / group : 0) - pos);
                         s[n][0] = g < n0 ? s[n][0] * f0 : -INFINITY;
                         s[n][1] = g < n1 ? s[n][1] * f1 : -INFINITY;
                         s[n][2] = g + 8 < n0 ? s[n][2] * f0 : -INFINITY;

@@ -27,7 +27,7 @@ from .runtime import Context
 
 ROOT = Path(__file__).resolve().parent.parent
 
-OPS = ["prefill", "rms_norm", "rms_norm_bwd", "rotary", "rope_copy_kv", "penalty", "copy_kv", "qk", "pv", "pair", "decode", "paged"]
+OPS = ["prefill", "rms_norm", "rms_norm_bwd", "rotary", "rope_copy_kv", "penalty", "copy_kv", "qk", "pv", "pair", "decode", "paged", "paged_quant", "copy_quant"]
 
 
 def peaks():
@@ -271,6 +271,29 @@ def run_op(op: str, size: str = "full", iters: int = 10, warmup: int = 3, kv_hea
         rec.update(ms=back, bytes=nbytes, gbs=nbytes / back / 1e6, frac_of_peak=nbytes / back / 1e6 / hbm, unit="GB/s", q_heads=c["q_heads"], kv_heads=kv_heads,
                    sum_len=c["sum_len"], note="bytes = every K/V row once + q + out: the figure a single pass over the rows is bound by",
                    timing="launches queued back to back, average per call")
+    elif op in ("paged_quant", "copy_quant"):
+        # The batch of "paged" with its cache in 8 bits (e4m3): the store of all its tokens as one prefill, then the decode
+        # attention over what it wrote. diopiQuantizedCopyKV and diopiQuantizedPagedAttention.
+        c = paged_case(kv_heads) if size == "full" else paged_case(kv_heads, B=16)
+        B, D, block, blocks = len(c["lens"]), c["D"], c["block"], c["k"].shape[0] // c["block"]
+        cache = [torch.zeros(blocks, block, kv_heads, D, dtype=torch.float8_e4m3fn, device="cuda") for _ in range(2)]
+        scale = [torch.zeros(blocks, kv_heads, device="cuda") for _ in range(2)]
+        lens = torch.tensor(c["lens"], dtype=torch.int32, device="cuda")
+        zeros = torch.zeros_like(lens)
+        starts = torch.cat([zeros[:1], lens.cumsum(0)]).to(torch.int32)
+        rows = [c[x][:c["sum_len"]].view(-1, kv_heads, D) for x in ("k", "v")]   # any rows do: the values are random
+        store = lambda: F.quantized_copy_kv(*rows, c["table"], zeros, starts, *cache, *scale, ctx=ctx)  # noqa: E731
+        store()
+        q = c["q"].view(B, c["q_heads"], D)
+        out = torch.empty_like(q)
+        attend = lambda: (F.quantized_paged_attention(q, *cache, *scale, c["table"], lens, D ** -0.5, out=out, ctx=ctx), ctx.release())  # noqa: E731
+        with sampler:
+            back = time_rotating([attend if op == "paged_quant" else store], rounds=max(20, iters), warmup=max(2, warmup))
+        codes = 2 * c["sum_len"] * kv_heads * D
+        scales = 2 * 4 * kv_heads * c["sum_len"] // block
+        nbytes = codes + scales + (2 * c["q"].numel() * 2 if op == "paged_quant" else 2 * codes)
+        rec.update(ms=back, bytes=nbytes, gbs=nbytes / back / 1e6, frac_of_peak=nbytes / back / 1e6 / hbm, unit="GB/s", q_heads=c["q_heads"], kv_heads=kv_heads,
+                   sum_len=c["sum_len"], code="e4m3", timing="launches queued back to back, average per call")
     elif op == "penalty":
         p = workloads.penalty()
         flush = _flush_buffer()
@@ -320,7 +343,7 @@ def main():
     ap.add_argument("--size", default="full", choices=["full", "small"])
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--warmup", type=int, default=3)
-    ap.add_argument("--kv-heads", type=int, default=8, help="paged: K/V heads under 64 query heads")
+    ap.add_argument("--kv-heads", type=int, default=8, help="paged, paged_quant, copy_quant: K/V heads under 64 query heads")
     ap.add_argument("--head-dim", type=int, default=128, help="prefill: head dimension (heads = 4096 / head_dim)")
     ap.add_argument("--compare", action="store_true", help="prefill: also time installed library attention kernels on the same batch")
     args = ap.parse_args()

@@ -592,6 +592,120 @@ def test_attention_on_another_stream_and_in_a_graph(F):
             assert bool(((out.cpu().double() - want).abs() <= bound_of(want, sums, 1000, 128, q.dtype)).all())
 
 
+def test_which_kernel_takes_a_call(F, ctx, capfd):
+    """The split kernel wherever width and block size are multiples of 16 and the cache's rows are aligned."""
+    F.set_option("log", 1)
+    try:
+        for kw, kernel in ((dict(), "split"), (dict(D=16), "split"), (dict(D=256, dt="fp32"), "split"), (dict(bs=48), "split"), (dict(bs=24), "plain"), (dict(D=40), "plain"),
+                           (dict(D=272), "plain"), (dict(n=3, group=50), "split")):
+            args = [t.cuda() for t in attention_inputs([70, 3], **kw)]
+            capfd.readouterr()
+            F.quantized_paged_attention(*args, 0.1, ctx=ctx)
+            assert f"({kernel} kernel)" in capfd.readouterr().err, kw
+    finally:
+        F.set_option("log", 0)
+
+
+@pytest.mark.parametrize("Hkv,group,D", [(1, 300, 64), (2, 129, 128), (1, 64, 256)])
+def test_attention_of_wide_groups(F, ctx, Hkv, group, D):
+    """More query rows on a K/V head than the warps of a CTA take."""
+    check_attention(F, ctx, attention_inputs([300, 0, 17], Hkv=Hkv, group=group, D=D, dt="fp16"))
+
+
+def test_attention_of_thousands_of_requests(F, ctx):
+    g = torch.Generator().manual_seed(2)
+    lens = torch.randint(0, 20, (4100,), generator=g).tolist()   # more than the split kernel keeps the lengths of
+    check_attention(F, ctx, attention_inputs(lens, D=64, Hkv=1, group=2, dt="fp16"))
+    check_attention(F, ctx, attention_inputs(lens[:4096], D=64, Hkv=1, group=2, dt="fp16"))
+
+
+def test_the_next_operation_finds_the_output(F, ctx):
+    """Requests that need no merge: the second kernel of a call must not end the call before the first one has."""
+    args = [t.cuda() for t in attention_inputs([60] * 40, D=128, Hkv=8, group=2)]
+    want = F.quantized_paged_attention(*args, 0.1, ctx=ctx)
+    out = torch.empty_like(want)
+    for _ in range(200):
+        ctx.release()
+        out.fill_(7.0)
+        F.quantized_paged_attention(*args, 0.1, ctx=ctx, out=out)
+        assert torch.equal(out.clone(), want)
+
+
+def test_calls_on_two_streams_at_once(F):
+    """Each stream has a context, hence scratch, of its own."""
+    from diopi_b200.runtime import Context
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    args = [[t.cuda() for t in attention_inputs([2000, 31, 700], seed=s)] for s in range(2)]
+    wants = [F.quantized_paged_attention(*a, 0.1, ctx=Context()) for a in args]
+    ctxs = [Context(st) for st in streams]
+    outs = [[torch.empty_like(w) for _ in range(30)] for w in wants]
+    torch.cuda.synchronize()
+    for i in range(30):
+        for s in range(2):
+            with torch.cuda.stream(streams[s]):
+                F.quantized_paged_attention(*args[s], 0.1, ctx=ctxs[s], out=outs[s][i])
+                ctxs[s].release()
+    torch.cuda.synchronize()
+    for s in range(2):
+        assert all(torch.equal(o, wants[s]) for o in outs[s])
+
+
+def test_a_captured_step_of_all_three(F):
+    """Tables, store and attention in one graph, replayed with other lengths: a decode loop without the host."""
+    from diopi_b200.runtime import Context
+    g = torch.Generator().manual_seed(9)
+    B, H, Hkv, D, bs, cols = 4, 8, 2, 64, 16, 6
+    i32 = dict(dtype=torch.int32, device="cuda")
+    blocks = B * cols
+    start_lens = torch.tensor([5, 0, 16, 40])
+    o_table = paged(B, start_lens.tolist(), bs, cols, blocks, g)
+    o_table = torch.where(o_table > blocks, torch.full_like(o_table, -1), o_table)
+    used = set(o_table[o_table >= 0].tolist())
+    free = torch.tensor([b for b in range(blocks) if b not in used])
+    table, d_free, at, nxt = o_table.to(**i32), free.to(**i32), torch.zeros(1, **i32), torch.zeros(1, **i32)
+    cached, new, seq, starts, slots = start_lens.to(**i32), torch.ones(B, **i32), torch.zeros(B, **i32), torch.zeros(B + 1, **i32), torch.zeros(B, **i32)
+    o_cache = [random_codes((blocks, bs, Hkv, D), True, g) for _ in range(2)]
+    o_scale = [torch.full((blocks, Hkv), 0.125) for _ in range(2)]
+    cache, scale = [c.cuda() for c in o_cache], [s.cuda() for s in o_scale]
+    k, v, q = [torch.zeros(B, h, D, dtype=torch.float16, device="cuda") for h in (Hkv, Hkv, H)]
+    out = torch.zeros_like(q)
+    st = torch.cuda.Stream()
+    ctx = Context(st)
+
+    def step():
+        F.build_block_table(table, cached, new, d_free, at, bs, slot_map=slots, new_start=starts, seq_lens=seq, free_next=nxt, ctx=ctx)
+        F.quantized_copy_kv(k, v, table, cached, starts, *cache, *scale, ctx=ctx)
+        F.quantized_paged_attention(q, *cache, *scale, table, seq, 0.125, out=out, ctx=ctx)
+
+    keep = [t.clone() for t in (table, *cache, *scale)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        step()                       # sizes the scratch outside the capture
+        st.synchronize()
+        ctx.release()
+        for t, was in zip((table, *cache, *scale), keep):
+            t.copy_(was)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            step()
+            cached.copy_(seq)
+            at.copy_(nxt)
+        o_cached, o_at = start_lens, 0
+        for _ in range(20):
+            hk, hv, hq = [torch.randn(t.shape, generator=g).half() for t in (k, v, q)]
+            k.copy_(hk), v.copy_(hv), q.copy_(hq)
+            graph.replay()
+            st.synchronize()
+            o_table, _, o_starts, o_lens, o_at, _ = O.build_block_table(o_table, o_cached, torch.ones(B, dtype=torch.int64), free, o_at, bs, B)
+            for m, x in enumerate((hk, hv)):
+                o_cache[m], o_scale[m] = O.quantized_copy(x, o_table, o_cached, o_starts, o_cache[m], o_scale[m])
+                assert torch.equal(cache[m].cpu(), o_cache[m]) and torch.equal(scale[m].cpu(), o_scale[m])
+            want, sums = O.quantized_paged_attention(hq[:, None], *o_cache, *o_scale, o_table, o_lens, 0.125)
+            assert bool(((out.cpu().double()[:, None] - want).abs() <= bound_of(want, sums, 96, D, torch.float16)).all())
+            o_cached = o_lens
+    assert take_status(F) is None
+
+
 # ---------------------------------------------------------------------------------------------------
 # the three together
 # ---------------------------------------------------------------------------------------------------

@@ -149,3 +149,38 @@ def test_host_tensors_are_refused(F):
     c = cache_args()
     with pytest.raises(DiopiError, match="host memory"):
         F.quantized_copy_kv(*c.values(), as_device=False)
+
+
+# ---- the call from Python ---------------------------------------------------------------------------
+class ElsewhereTensor:
+    """What a call looks at of a tensor, on the second device."""
+    dtype, shape = torch.int32, (1,)
+
+    def stride(self):
+        return (1,)
+
+    def data_ptr(self):
+        return 4096
+
+    def get_device(self):
+        return 1
+
+
+def test_tensors_of_another_device_are_refused(F):
+    a, kw = table_args()
+    with pytest.raises(ValueError, match="cuda:1"):
+        F.build_block_table(ElsewhereTensor(), *list(a.values())[1:], **kw)
+
+
+def test_what_a_call_takes(F, built_libs):
+    """Handles made beforehand, None where a tensor may be missing, no other type; a dtype without a counterpart is an error."""
+    from diopi_b200.runtime import Tensor
+    c = cache_args()
+    c["k_cache"] = Tensor(c["k_cache"], as_device=True)
+    c["v_scale"] = Tensor(torch.zeros(6, 5), as_device=True)
+    fails(ERROR_OCCURRED, F.quantized_copy_kv, *c.values(), match="'v_scale' must be")
+    with pytest.raises(TypeError, match="complex"):
+        F.quantized_copy_kv(*{**cache_args(), "k": torch.zeros(5, 4, 32, dtype=torch.complex64)}.values(), as_device=True)
+    with pytest.raises(AttributeError):
+        F.quantized_copy_kv(*{**cache_args(), "k": [1, 2]}.values(), as_device=True)
+    fails(ERROR_OCCURRED, F.quantized_copy_kv, *{**cache_args(), "k": torch.zeros([1] * 9)}.values(), match="at most 8")
