@@ -9,9 +9,11 @@
 // the work gives the same bits. NaN and infinities do not count into amax: they saturate (int8 NaN: 0, e4m3 NaN: NaN).
 //
 // Bytes: T * H * D * (e + 1) for each of K and V. One pass: the rows of a block stay in registers between the maximum and
-// the codes. A unit is one (request, block, head) of one matrix; 16 rows of it belong to a warp, with 16 elements of a row to
-// a lane, and ceil(block_size / 16) warps (up to 8) share a unit through shared memory. Blocks
-// of more than 128 rows are read twice (the second time from L1/L2).
+// the codes. A unit is one (request, block, head) of one matrix; 16 (8) rows of it belong to a warp, with 16 elements of a row to
+// a lane, and up to 8 warps share a unit through shared memory. Blocks of more rows than that are read twice (the second time from
+// L1/L2). Bound by memory latency over 24 warps an SM, then by its rate: 36864 tokens x 32 heads x 128, fp16 to int8: 171 us =
+// 5300 GB/s = 0.81 of the copy rate; 124971 tokens x 8 heads, fp16 to e4m3: 132 us, 0.89. On the way there: vectors side by side
+// in a lane instead of whole lines, 394 us; calls for the rare cases inside the loop (spills), 231.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -24,7 +26,6 @@ namespace {
 
 constexpr int kCopyThreads = 256;
 constexpr int kCopyWarps = kCopyThreads / 32;
-constexpr int kWarpRows = 16;
 constexpr float kFltMin = 1.17549435e-38f;   // 2^-126
 
 // The scale of a block that begins anew.
@@ -211,9 +212,16 @@ __device__ __forceinline__ float finite_top_of(const uint4& v) {
 
 constexpr uint32_t kInfBits = 0x7f800000u;
 
-// CTAs of an SM that the registers are to leave room for: the rows of a warp's 16 are held between the two passes.
+// Rows of a warp: 16, or 8 where 16 of them would take 64 registers of every lane in fp32 (19 requests of up to 517 tokens, 5
+// heads x 80: 12.7 us; 13.7 with 16).
 template <typename T>
-constexpr int copy_ctas(int lpr) { return sizeof(T) * lpr <= 8 ? 4 : sizeof(T) * lpr <= 16 ? 3 : sizeof(T) * lpr <= 32 ? 2 : 1; }
+constexpr int warp_rows(int lpr) { return sizeof(T) == 4 && lpr >= 8 ? 8 : 16; }
+// CTAs of an SM that the registers are to leave room for: the rows are held between the two passes.
+template <typename T>
+constexpr int copy_ctas(int lpr) {
+    const int held = warp_rows<T>(lpr) * lpr / 32 * 4 * static_cast<int>(sizeof(T));   // registers of a lane
+    return held <= 16 ? 4 : held <= 32 ? 3 : held <= 64 ? 2 : 1;
+}
 
 // One row of a unit with a NaN or an infinity in it; the lanes of a row share it.
 template <typename T, bool E4M3>
@@ -241,12 +249,13 @@ __device__ __noinline__ void shrink_rows(uint8_t* dst, int64_t pitch, int p, int
 }
 
 // Lanes of a row LPR, with 16 elements each: vectors of 16 bytes, LPR lanes apart, so that a load covers whole lines (where the
-// row is shorter some vectors are left out). W warps of 16 rows to a unit.
+// row is shorter some vectors are left out). W warps to a unit.
 template <typename T, bool E4M3, int LPR, int W, bool REREAD>
 __global__ void __launch_bounds__(kCopyThreads, copy_ctas<T>(LPR)) quantized_copy_kernel(const QuantCopyArgs a) {
     constexpr int E = Vec16<T>::N;             // elements of a vector
     constexpr int N = 16 / E;                  // vectors of a lane's row
     constexpr int RPP = 32 / LPR;              // rows of a warp's pass
+    constexpr int kWarpRows = warp_rows<T>(LPR);
     constexpr int PASSES = kWarpRows / RPP;
     constexpr int UPC = kCopyWarps / W;        // heads of a CTA
     __shared__ uint32_t s_top[2][kCopyWarps];
@@ -418,13 +427,15 @@ void launch_rows(const QuantCopyArgs& a, int units, int sm_count, cudaStream_t s
     auto go = [&](auto kern, int w) {
         const int upc = kCopyWarps / w;
         const int y = (a.H + upc - 1) / upc;
-        // Few CTAs: K and V side by side (64 requests of one token: 6.2 us; 8.0 one after the other); many: one look-up for both.
+        // Few CTAs: K and V side by side (64 requests of one token: 3.7 us, 4.8 one after the other); many: one look-up for both
+        // (the prompts above: 171 us, 198 side by side).
         kern<<<dim3(units, y, static_cast<int64_t>(units) * y < 8 * sm_count ? 2 : 1), kCopyThreads, 0, st>>>(a);
     };
-    if (a.block_size <= 16) go(quantized_copy_kernel<T, E4M3, LPR, 1, false>, 1);
-    else if (a.block_size <= 32) go(quantized_copy_kernel<T, E4M3, LPR, 2, false>, 2);
-    else if (a.block_size <= 64) go(quantized_copy_kernel<T, E4M3, LPR, 4, false>, 4);
-    else if (a.block_size <= 128) go(quantized_copy_kernel<T, E4M3, LPR, 8, false>, 8);
+    constexpr int rows = warp_rows<T>(LPR);
+    if (a.block_size <= rows) go(quantized_copy_kernel<T, E4M3, LPR, 1, false>, 1);
+    else if (a.block_size <= 2 * rows) go(quantized_copy_kernel<T, E4M3, LPR, 2, false>, 2);
+    else if (a.block_size <= 4 * rows) go(quantized_copy_kernel<T, E4M3, LPR, 4, false>, 4);
+    else if (a.block_size <= 8 * rows) go(quantized_copy_kernel<T, E4M3, LPR, 8, false>, 8);
     else go(quantized_copy_kernel<T, E4M3, LPR, 8, true>, 8);
 }
 
