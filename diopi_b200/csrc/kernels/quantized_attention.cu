@@ -3,10 +3,10 @@
 //     x_j = softmax_scale * ks[b_j] * (q . kc_j),   out = sum_j softmax(x)_j * vs[b_j] * vc_j
 // New token t of n sees the first L - (n - 1 - t) tokens; a row that sees none gives zeros.
 //
-// quant_split_kernel (block_size and head_dim multiples of 16, head_dim up to 256) is bound by the bytes of the codes. The
+// quant_split_kernel (head_dim a multiple of 16 up to 256, any block_size) is bound by the bytes of the codes. The
 // query rows that share a K/V head (n * group of them) are the N extent of mma.sync m16n8k16 in fp16 with fp32
 // accumulators: every code of either kind is an fp16 number, so nothing is lost by the conversion in registers, and the
-// scales stay outside the products. A tile is 16 tokens of one K/V head, always inside one block, hence one ks and one vs:
+// scales stay outside the products. A tile is up to 16 tokens of one K/V head, always inside one block, hence one ks and one vs:
 //     S^T = Kc Q^T;  m = max(S f), f = ks * softmax_scale * log2 e;  P = 2^(S f - m + 15);  O^T += (2^(m - ref) vs) (Vc^T P^T)
 // The weights are taken against the tile's own maximum, so that they fill fp16's range (2^15 down to 2^-24: what is lost is
 // below 2^-40 of the tile's largest weight) whatever the other tiles hold, and the product of a tile is added in fp32 with
@@ -57,6 +57,15 @@ __device__ __forceinline__ int quant_len(const QuantAttnArgs& a, int i) {
     const int64_t cap = static_cast<int64_t>(a.cols) * a.block_size;
     const int64_t L = load_index(a.lens, i);
     return static_cast<int>(imin64(imax64(L, 0), cap));
+}
+
+constexpr int kTile = 16;   // tokens of a tile
+
+// Tiles of L tokens: none reaches over the end of a block.
+__device__ __forceinline__ int tiles_of(const QuantAttnArgs& a, int L) {
+    if (a.block_size % kTile == 0) return (L + kTile - 1) / kTile;
+    const int full = L / a.block_size, rest = L - full * a.block_size;
+    return full * ((a.block_size + kTile - 1) / kTile) + (rest + kTile - 1) / kTile;
 }
 
 constexpr int kPlainWarps = 4;
@@ -140,7 +149,6 @@ __global__ void __launch_bounds__(32 * kPlainWarps) quant_plain_kernel(const Qua
 // ---------------------------------------------------------------------------------------------------
 constexpr int kQMaxStages = 8;
 constexpr int kQMaxB = 4096;
-constexpr int kTile = 16;                       // tokens of a tile
 constexpr int kTilesPerRange = 4;               // at least, so that short batches are not cut into crumbs (2: the same times, twice the parts)
 
 // Warps of a CTA: as many as the registers of a thread's queries and accumulators leave room for (a spilled register costs
@@ -155,6 +163,8 @@ struct QuantPlan {
     int hw;           // K/V heads of a CTA: a divisor of Hkv
     int n_hg;         // CTAs along the K/V heads
     int tw;           // ranges of a CTA
+    int block_tiles;  // tiles of a block
+    bool ragged;      // the last of them is not full
     int stages;       // tiles of a team's ring
     int n_cta, n_range;
     int off_bars, off_pre, off_len, off_flag, smem_bytes;
@@ -249,7 +259,7 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
     for (int i = tid; i < a.B; i += kThreads) {
         const int L = quant_len(a, i);
         lens[i] = L;
-        pre[i + 1] = (L + kTile - 1) / kTile;
+        pre[i + 1] = tiles_of(a, L);
     }
     __syncthreads();
     if (warp == 0) {
@@ -295,14 +305,21 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
             }
             return lo;
         };
+        // First position of a request's tile, its block's column and its place in the block.
+        auto place_of = [&](int tile, int& col, int& at) {
+            col = tile / p.block_tiles;
+            at = (tile - col * p.block_tiles) * kTile;
+            return col * a.block_size + at;
+        };
         // In two halves, so that what comes between them hides the load of the block ids.
         auto ask_ids = [&](Ahead& x, int from) -> int64_t {
             x.at = 0;
             const int t = from + lane;
             if (t >= t1) return 0;
             const int i = request_of(t);
-            const int pos = (t - pre[i]) * kTile, col = pos / a.block_size;
-            x.at = (pos - col * a.block_size) * 32 + min(kTile, lens[i] - pos);
+            int col, at;
+            const int pos = place_of(t - pre[i], col, at);
+            x.at = at * 32 + min(min(kTile, a.block_size - at), lens[i] - pos);
             return load_index(a.table, i, col);
         };
         auto take_ids = [&](Ahead& x, int64_t id) {
@@ -530,7 +547,8 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                 }
                 // ---- weights against the tile's own maximum ----
                 // s[0], s[1]: token g, rows 2c, 2c + 1; s[2], s[3]: token g + 8
-                const int pos = (t - pre[req]) * kTile;
+                int col, at, pos = (t - pre[req]) * kTile;
+                if (p.ragged) pos = place_of(t - pre[req], col, at);
                 const bool whole = valid == kTile && pos + kTile <= lim_min;
                 uint32_t pb[NT][2], pl[NT][2];
                 float gain[NT][2];
@@ -711,7 +729,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps, U > 4 ? 1 : HD > 128 ? 3 : 4
     const int i = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int before = 0, all = 0;
     for (int r = threadIdx.x; r < a.B; r += 32 * kMergeWarps) {
-        const int n = (quant_len(a, r) + kTile - 1) / kTile;
+        const int n = tiles_of(a, quant_len(a, r));
         all += n;
         if (r < i) before += n;
     }
@@ -731,7 +749,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps, U > 4 ? 1 : HD > 128 ? 3 : 4
         before += s_part[w][0];
         all += s_part[w][1];
     }
-    const int tiles = (quant_len(a, i) + kTile - 1) / kTile;
+    const int tiles = tiles_of(a, quant_len(a, i));
     const int used = used_ranges(all, n_range);
     // Range c has the tiles [all * c / used, all * (c + 1) / used): every one of the used ranges has some.
     int c_first = 0, parts = 0;
@@ -838,7 +856,7 @@ EncodeFn encode_fn() {
 }
 
 // [head_dim, position, head, block] of one cache whatever its strides; a box is 16 positions of a head. Bytes of a row
-// beyond head_dim arrive as zeros.
+// beyond head_dim and rows beyond the block arrive as zeros.
 bool encode_map(const QuantAttnArgs& a, const QuantPlan& p, int m, CUtensorMap* map) {
     EncodeFn fn = encode_fn();
     if (!fn) return false;
@@ -855,9 +873,10 @@ bool encode_map(const QuantAttnArgs& a, const QuantPlan& p, int m, CUtensorMap* 
 
 // Whether the split kernel takes these arguments, and how it cuts them.
 bool make_quant_plan(const QuantAttnArgs& a, int sm_count, int max_smem, QuantPlan& p) {
-    if (a.force_plain || a.D % 16 != 0 || a.block_size % kTile != 0 || a.blocks <= 0 || a.cols <= 0) return false;
+    if (a.force_plain || a.D % 16 != 0 || a.block_size >= (1 << 25) || a.blocks <= 0 || a.cols <= 0) return false;
     if (a.D > 256) return false;
-    if (a.B > kQMaxB || static_cast<int64_t>(a.B) * a.cols * a.block_size / kTile >= (1ll << 30) || a.blocks >= (1ll << 31)) return false;
+    const int64_t block_tiles = (a.block_size + kTile - 1) / kTile;
+    if (a.B > kQMaxB || static_cast<int64_t>(a.B) * a.cols * block_tiles >= (1ll << 30) || a.blocks >= (1ll << 31)) return false;
     for (int m = 0; m < 2; ++m) {
         auto ok = [](int64_t s, int64_t extent) { return extent <= 1 || (s > 0 && s % 16 == 0 && s < (1ll << 40)); };
         if (a.c_s3[m] != 1 || !ok(a.c_s0[m], a.blocks) || !ok(a.c_s1[m], a.block_size) || !ok(a.c_s2[m], a.Hkv) ||
@@ -865,6 +884,8 @@ bool make_quant_plan(const QuantAttnArgs& a, int sm_count, int max_smem, QuantPl
             return false;
     }
     p = QuantPlan{};
+    p.block_tiles = static_cast<int>(block_tiles);
+    p.ragged = a.block_size % kTile != 0;
     p.hd = a.D <= 64 ? 64 : a.D <= 128 ? 128 : 256;
     const int R = a.n * (a.Hq / a.Hkv);
     const bool f32 = a.dt == Dt::F32;
@@ -899,7 +920,7 @@ bool make_quant_plan(const QuantAttnArgs& a, int sm_count, int max_smem, QuantPl
     p.off_flag = take(4);
     p.smem_bytes = off + 1024;
     if (p.smem_bytes > max_smem) return false;
-    const int64_t most = static_cast<int64_t>(a.B) * ((static_cast<int64_t>(a.cols) * a.block_size + kTile - 1) / kTile);
+    const int64_t most = static_cast<int64_t>(a.B) * a.cols * block_tiles;
     const int64_t ranges = std::max<int64_t>(1, (most + kTilesPerRange - 1) / kTilesPerRange);
     p.n_cta = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count / (p.n_hg * p.n_z), (ranges + p.tw - 1) / p.tw)));
     p.n_range = p.n_cta * p.tw;

@@ -402,10 +402,28 @@ def test_attention_head_layouts(F, ctx, Hkv, group):
     check_attention(F, ctx, attention_inputs([0, 1, 40, 333, 16, 129], Hkv=Hkv, group=group, D=64, dt="fp16", seed=Hkv * 100 + group))
 
 
-@pytest.mark.parametrize("bs", [1, 8, 24, 32, 48, 64, 128, 272])
+@pytest.mark.parametrize("bs", [1, 3, 8, 17, 24, 32, 48, 64, 100, 128, 272])
 @pytest.mark.parametrize("e4m3", [True, False])
 def test_attention_block_sizes(F, ctx, bs, e4m3):
-    check_attention(F, ctx, attention_inputs(LENS + [bs, bs + 1, 2 * bs - 1], bs=bs, D=64, e4m3=e4m3, seed=bs), idx=torch.int64)
+    args = attention_inputs(LENS + [bs, bs + 1, 2 * bs - 1], bs=bs, D=64, e4m3=e4m3, seed=bs)
+    check_attention(F, ctx, args, idx=torch.int64)
+    check_attention(F, ctx, attention_inputs(LENS + [bs, 700], bs=bs, D=128, e4m3=e4m3, seed=bs, n=3, group=3))
+
+
+@pytest.mark.parametrize("bs", [8, 24, 40])
+def test_attention_ignores_the_next_block(F, ctx, bs):
+    """Blocks that do not fill a tile: what lies behind a block in memory (NaN here) is another block's."""
+    lens = [bs, 3 * bs - 1, 5, 0]
+    q, kc, vc, ks, vs, table, lens_t = attention_inputs(lens, D=64, bs=bs, dt="fp16")
+    used = torch.cat([table[i, :-(-L // bs)] for i, L in enumerate(lens)])
+    keep = [c[used].clone() for c in (kc, vc)]
+    for c, k in zip((kc, vc), keep):
+        c[:] = 0x7f
+        c[used] = k
+        for i, L in enumerate(lens):
+            if L % bs:
+                c[table[i, L // bs], L % bs:] = 0x7f
+    check_attention(F, ctx, (q, kc, vc, ks, vs, table, lens_t))
 
 
 @pytest.mark.parametrize("n", [2, 3, 5, 16])
@@ -491,8 +509,8 @@ def test_attention_strides(F, ctx, e4m3):
 
 
 def test_attention_leaves_out_blocks_outside_the_cache(F, ctx):
-    for bs in (16, 8):
-        q, kc, vc, ks, vs, table, lens = attention_inputs([100, 40, 30], D=64, bs=bs)
+    for bs, D in ((16, 64), (8, 64), (16, 40)):
+        q, kc, vc, ks, vs, table, lens = attention_inputs([100, 40, 30], D=D, bs=bs)
         table[0, 2], table[1, 0], table[2] = -1, kc.shape[0], 1 << 30
         got = check_attention(F, ctx, (q, kc, vc, ks, vs, table, lens))
         assert bool((got[2] == 0).all())
@@ -593,10 +611,10 @@ def test_attention_on_another_stream_and_in_a_graph(F):
 
 
 def test_which_kernel_takes_a_call(F, ctx, capfd):
-    """The split kernel wherever width and block size are multiples of 16 and the cache's rows are aligned."""
+    """The split kernel wherever the width is a multiple of 16 up to 256 and the cache's rows are aligned."""
     F.set_option("log", 1)
     try:
-        for kw, kernel in ((dict(), "split"), (dict(D=16), "split"), (dict(D=256, dt="fp32"), "split"), (dict(bs=48), "split"), (dict(bs=24), "plain"), (dict(D=40), "plain"),
+        for kw, kernel in ((dict(), "split"), (dict(D=16), "split"), (dict(D=256, dt="fp32"), "split"), (dict(bs=48), "split"), (dict(bs=24), "split"), (dict(bs=1), "split"), (dict(D=40), "plain"),
                            (dict(D=272), "plain"), (dict(n=3, group=50), "split")):
             args = [t.cuda() for t in attention_inputs([70, 3], **kw)]
             capfd.readouterr()
