@@ -352,15 +352,17 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
         const int rbase = (blockIdx.z * p.mt + mtile) * 8 * NT;   // first query row of this warp
         // K: lane l names row l & 7 of matrix l >> 3, matrix m being the 16 bytes 4 i + m of eight tokens. In each register the lane
         // then has four neighbouring codes of token g: k columns 2c, 2c + 1 and 2c + 8, 2c + 9 of a k step stand for d = 4c .. 4c + 3.
-        const int krow = lane & 7, ksw = RB == 128 ? krow : (krow >> 1);
+        // The swizzle moves the 16 bytes i of a row to i ^ (row & 7), or (row / 2) & 3 in rows of 64 bytes; tiles start at
+        // multiples of 1024 bytes, so a change of i or of the row's parity is a change of address bits.
+        const uint32_t k_lane = (lane & 7) * RB + (((lane >> 3) ^ (RB == 128 ? lane & 7 : (lane & 7) >> 1)) << 4);
         // V: the lane has VB neighbouring codes, at d = VB * g, of tokens 2c, 2c + 1, 2c + 8, 2c + 9: the k columns that its A
         // fragments want. Rows g and g + 8 of M tile j stand for d = VB * g + 2 j and the next one.
-        const uint32_t v_lane = static_cast<uint32_t>(NH * BOX + 2 * c * RB);
+        const uint32_t v_lane = NH * BOX + 2 * c * RB + (RB == 128 ? (g ^ (2 * c)) << 4 : (((g >> 1) ^ c) << 4) + (g & 1) * 8);
 
         uint32_t qf[NT][CH][2], ql[NT][SPLIT ? CH : 1][2];
         float o[NT][DM][4];                             // rows 2c (elements 0, 2) and 2c + 1 (1, 3) of the N tile
         float ref[NT][2], l[NT][2], rs[NT][2];
-        int req = request_of(t0) - 1, req_end = t0, part_first = 0, lim_min = 0;
+        int req = request_of(t0) - 1, req_end = t0, part_first = 0, lim_min = 0, whole_end = 0;
         // The next request from tile t on: its query rows as they are in memory ...
         auto ask_request = [&](int t) {
             do ++req;
@@ -368,6 +370,8 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
             req_end = min(pre[req + 1], t1);
             part_first = t - pre[req];
             lim_min = lens[req] - (a.n - 1);            // what the first new token sees
+            // Full tiles before this one are seen by every row: with one new token all of them.
+            whole_end = a.n == 1 ? t1 : pre[req] + (p.ragged ? 0 : max(lim_min, 0) / kTile);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 // ---- query row g of the N tile as a B fragment ----
@@ -492,8 +496,7 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                 for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.f;
 #pragma unroll
                 for (int i = 0; i < CH; i += 4) {
-                    const int cc = (i % (RB / 16)) + (lane >> 3);
-                    const uint32_t at = kt + (i * 16 / RB) * BOX + krow * RB + ((cc ^ ksw) << 4);
+                    const uint32_t at = ((kt + k_lane) ^ (i % (RB / 16) * 16)) + (i * 16 / RB) * BOX;
                     uint32_t b[4], d[4];
                     ldmatrix4(at, b);            // tokens 0-7
                     ldmatrix4(at + 8 * RB, d);   // tokens 8-15
@@ -518,18 +521,18 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                 uint32_t v[NH][4][VB / 4];   // tokens 2c, 2c + 1, 2c + 8, 2c + 9
 #pragma unroll
                 for (int h = 0; h < NH; ++h) {
-                    const uint32_t vb = kt + h * BOX + v_lane;
+                    const uint32_t vb = kt + v_lane;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint32_t trow = (i & 1) * RB + (i >> 1) * 8 * RB;
+                        const uint32_t trow = (i & 1) * RB + (i >> 1) * 8 * RB + h * BOX;
                         if constexpr (RB == 128) {
-                            const uint32_t at = vb + trow + ((g ^ (2 * c + (i & 1))) << 4);
+                            const uint32_t at = (vb ^ ((i & 1) << 4)) + trow;
                             asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                                          : "=r"(v[h][i][0]), "=r"(v[h][i][1]), "=r"(v[h][i][2]), "=r"(v[h][i][3])
                                          : "r"(at)
                                          : "memory");
                         } else {
-                            const uint32_t at = vb + trow + (((g >> 1) ^ c) << 4) + (g & 1) * 8;
+                            const uint32_t at = vb + trow;
                             asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[h][i][0]), "=r"(v[h][i][1]) : "r"(at) : "memory");
                         }
                     }
@@ -547,9 +550,12 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                 }
                 // ---- weights against the tile's own maximum ----
                 // s[0], s[1]: token g, rows 2c, 2c + 1; s[2], s[3]: token g + 8
-                int col, at, pos = (t - pre[req]) * kTile;
-                if (p.ragged) pos = place_of(t - pre[req], col, at);
-                const bool whole = valid == kTile && pos + kTile <= lim_min;
+                const bool whole = valid == kTile && t < whole_end;
+                int pos = 0;
+                if (!whole) {
+                    int col, at;
+                    pos = place_of(t - pre[req], col, at);
+                }
                 uint32_t pb[NT][2], pl[NT][2];
                 float gain[NT][2];
 #pragma unroll
