@@ -22,8 +22,8 @@
 // ranges its parts are merged by quant_combine_kernel (a programmatic dependent launch); else it is written directly.
 //
 // Measured (calls one after the other in a graph, merge included): 64 query heads over 8 K/V heads, 64 requests of 512 to 4096
-// tokens, e4m3: 71 us = 4300 GB/s; a K/V head for each of 32 query heads, int8: 213 us = 5680 GB/s = 0.87 of the copy rate; four
-// requests of 30011 to 131072 tokens: 72 us. While it streams the loop runs at the copy rate (the loads alone take as long); what
+// tokens, e4m3: 71 us = 4300 GB/s; a K/V head for each of 32 query heads, int8: 209 to 233 us on different GPUs = 0.79 to 0.88
+// of the copy rate; four requests of 30011 to 131072 tokens: 71 us. While it streams the loop runs at the copy rate (the loads alone take as long); what
 // is left is 5 us of start (lengths, block ids, first tiles), up to 9 us between the first SM's end and the last one's
 // (some groups of SMs get a tenth less bandwidth), 5 us of merge. Tried and dropped: query rows as the M extent (half of
 // the products on padding; 98 us); a producer warp beside 16 others (96 registers, spills: 124 us); the last eighth of each
@@ -217,7 +217,9 @@ __device__ __forceinline__ void codes_to_f16(uint32_t c, uint32_t& lo, uint32_t&
 
 __device__ __forceinline__ int used_ranges(int total, int n_range) { return max(1, min(n_range, (total + kTilesPerRange - 1) / kTilesPerRange)); }
 
-template <typename T, bool E4M3, int HD, int NT>
+// MANY: more than one new token to a request, so that the rows of a tile may see different tokens. (Only the care for NaN
+// goes by it: the masks written out for one token alone, the kernel for e4m3 at head_dim 128 spills and is 4 % slower.)
+template <typename T, bool E4M3, int HD, int NT, bool MANY>
 __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value, HD, NT), 1)
     quant_split_kernel(const QuantAttnArgs a, const QuantPlan p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        float* __restrict__ ws_acc, float* __restrict__ ws_ml) {
@@ -609,6 +611,47 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                         pl[n][1] = transpose8(pack_rest(p2, p3, h1));
                     }
                 }
+                // A weight of 0 does not keep a NaN code out of a sum. Where some rows see a token and others do not (the new
+                // tokens among themselves), NaN codes are taken out of the tile and handed to the rows that see them.
+                if constexpr (E4M3 && MANY) {
+                    if (!whole) {
+                        uint32_t found = 0;   // bit 7 of every byte that is 0x7f or 0xff
+#pragma unroll
+                        for (int h = 0; h < NH; ++h)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                for (int w = 0; w < VB / 4; ++w) found |= (v[h][i][w] & 0x7f7f7f7fu) + 0x01010101u;
+                        if (__any_sync(0xffffffffu, (found & 0x80808080u) != 0)) {
+                            uint32_t sees[NT][2];   // bit k: the row sees token k of the tile
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e)
+                                    sees[n][e] = (1u << max(min(valid, lim_min + (rbase + 8 * n + 2 * c + e) / group - pos), 0)) - 1u;
+#pragma unroll
+                            for (int h = 0; h < NH; ++h)
+#pragma unroll
+                                for (int j = 0; j < VB; ++j) {
+                                    const uint32_t byte = 0xffu << (8 * (j & 3));
+                                    uint32_t tokens = 0;   // those whose code at this place is NaN
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        if ((~v[h][i][j / 4] & byte & 0x7f7f7f7fu) == 0) {
+                                            tokens |= 1u << (2 * c + (i & 1) + (i >> 1) * 8);
+                                            v[h][i][j / 4] &= ~byte;
+                                        }
+                                    tokens |= __shfl_xor_sync(0xffffffffu, tokens, 1);
+                                    tokens |= __shfl_xor_sync(0xffffffffu, tokens, 2);
+#pragma unroll
+                                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                        for (int e = 0; e < 2; ++e)
+                                            if (tokens & sees[n][e]) o[n][h * (VB / 2) + j / 2][2 * (j & 1) + e] = __int_as_float(0x7fffffff);
+                                }
+                        }
+                    }
+                }
                 // ---- O^T += (w vs) (Vc^T P^T) ----
 #pragma unroll
                 for (int h = 0; h < NH; ++h) {
@@ -937,9 +980,9 @@ bool make_quant_plan(const QuantAttnArgs& a, int sm_count, int max_smem, QuantPl
 
 int64_t part_rows(const QuantAttnArgs& a, const QuantPlan& p) { return (static_cast<int64_t>(p.n_range) + a.B) * a.n * a.Hq; }
 
-template <typename T, bool E4M3, int HD, int NT>
+template <typename T, bool E4M3, int HD, int NT, bool MANY>
 void launch_split(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap& mk, const CUtensorMap& mv, float* acc, float* ml, int max_smem, cudaStream_t st) {
-    auto kern = quant_split_kernel<T, E4M3, HD, NT>;
+    auto kern = quant_split_kernel<T, E4M3, HD, NT, MANY>;
     constexpr int threads = 32 * split_warps(std::is_same<T, float>::value, HD, NT);
     // once per kernel and device: the call is not free, and the limit may as well be the device's
     static std::atomic<uint64_t> done{0};
@@ -967,10 +1010,16 @@ void launch_split(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap&
 template <typename T>
 void launch_split_t(const QuantAttnArgs& a, const QuantPlan& p, const CUtensorMap& mk, const CUtensorMap& mv, float* acc, float* ml, int max_smem, cudaStream_t st) {
     auto go = [&](auto e4m3, auto hd) {
+        auto rows = [&](auto nt) {
+            if constexpr (e4m3.value) {   // int8 has no NaN
+                if (a.n > 1) return launch_split<T, true, hd.value, nt.value, true>(a, p, mk, mv, acc, ml, max_smem, st);
+            }
+            launch_split<T, e4m3.value, hd.value, nt.value, false>(a, p, mk, mv, acc, ml, max_smem, st);
+        };
         if constexpr (!std::is_same<T, float>::value && hd.value <= 128) {
-            if (p.nt == 2) return launch_split<T, e4m3.value, hd.value, 2>(a, p, mk, mv, acc, ml, max_smem, st);
+            if (p.nt == 2) return rows(std::integral_constant<int, 2>{});
         }
-        launch_split<T, e4m3.value, hd.value, 1>(a, p, mk, mv, acc, ml, max_smem, st);
+        rows(std::integral_constant<int, 1>{});
     };
     auto widths = [&](auto e4m3) {
         if (p.hd == 64)

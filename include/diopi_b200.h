@@ -273,7 +273,7 @@ diopiError_t diopiQuantizedCopyKV(diopiContextHandle_t ctx, diopiTensorHandle_t 
 /* diopiQuantizedPagedAttention: decode attention over such a cache. q, out [B, H, D] or [B, n, H, D] (fp16, bf16, fp32;
  * H a multiple of Hkv): the n newest tokens of each request, whose K/V rows are in the cache already. seq_lens [B] counts
  * all tokens of a request; token t of n sees the first seq_lens[i] - (n - 1 - t) of them, causally, and one that sees none
- * gets zeros. out = softmax(softmax_scale * q k^T) v with softmax_scale > 0. Scales must not be negative. Tokens in a block
+ * gets zeros. out = softmax(softmax_scale * q k^T) v with softmax_scale > 0. Scales must be finite and not negative. Tokens in a block
  * outside the cache are left out (status 1). */
 diopiError_t diopiQuantizedPagedAttention(diopiContextHandle_t ctx, diopiTensorHandle_t out, diopiConstTensorHandle_t q, diopiConstTensorHandle_t k_cache,
                                           diopiConstTensorHandle_t v_cache, diopiConstTensorHandle_t k_scale, diopiConstTensorHandle_t v_scale,

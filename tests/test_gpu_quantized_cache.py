@@ -489,6 +489,28 @@ def test_attention_hands_nan_on(F, ctx):
     assert torch.equal(torch.isnan(got), bad)
 
 
+@pytest.mark.parametrize("D,group,n", [(64, 2, 3), (128, 1, 2), (128, 5, 4), (256, 2, 3), (40, 2, 3)])
+def test_attention_keeps_nan_from_the_tokens_before_it(F, ctx, D, group, n):
+    """A NaN value of a new token is seen by that token's rows and those after it, not by the rows of the tokens before it."""
+    lens = [40, 33, n, 18]
+    q, kc, vc, ks, vs, table, lens_t = attention_inputs(lens, D=D, Hkv=2, group=group, n=n, dt="fp32" if D == 64 else "bf16")
+    clean = vc.clone()
+    bad = torch.zeros(len(lens), n, 2 * group, D, dtype=torch.bool)
+    for i, (L, t, h, d) in enumerate(zip(lens, (n - 1, 0, n - 1, 1), (0, 1, 0, 1), (3, D - 1, 0, D // 2))):
+        pos = L - n + t
+        vc[table[i, pos // 16], pos % 16, h, d] = 0xff if i % 2 else 0x7f
+        clean[table[i, pos // 16], pos % 16, h, d] = 0
+        bad[i, t:, h * group:(h + 1) * group, d] = True
+    kc[table[3, 1], 1, 0, 5] = 0x7f          # the last token's key, of head 0
+    bad[3, n - 1:, :group] = True
+    got = F.quantized_paged_attention(q.cuda(), kc.cuda(), vc.cuda(), ks.cuda(), vs.cuda(), table.cuda(), lens_t.cuda(), 0.1, ctx=ctx).cpu()
+    assert torch.equal(torch.isnan(got), bad)
+    kc[table[3, 1], 1, 0, 5] = 0
+    want, sums = O.quantized_paged_attention(q, kc, clean, ks, vs, table, lens_t, 0.1)
+    ok = (got.double() - want).abs() <= bound_of(want, sums, 40, D, q.dtype)
+    assert bool((ok | bad).all())
+
+
 @pytest.mark.parametrize("e4m3", [True, False])
 def test_attention_strides(F, ctx, e4m3):
     """q as a slice of a fused projection, a head-major cache, scales inside a wider tensor, an odd offset of the cache."""
