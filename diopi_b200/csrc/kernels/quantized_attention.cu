@@ -7,7 +7,7 @@
 // query rows that share a K/V head (n * group of them) are the N extent of mma.sync m16n8k16 in fp16 with fp32
 // accumulators: every code of either kind is an fp16 number, so nothing is lost by the conversion in registers, and the
 // scales stay outside the products. A tile is up to 16 tokens of one K/V head, always inside one block, hence one ks and one vs:
-//     S^T = Kc Q^T;  m = max(S f), f = ks * softmax_scale * log2 e;  P = 2^(S f - m + 15);  O^T += (2^(m - ref) vs) (Vc^T P^T)
+//     S^T = Kc Q^T;  m = f max(S), f = ks * softmax_scale * log2 e;  P = 2^((S - max S) f + 15);  O^T += (2^(m - ref) vs) (Vc^T P^T)
 // The weights are taken against the tile's own maximum, so that they fill fp16's range (2^15 down to 2^-24: what is lost is
 // below 2^-40 of the tile's largest weight) whatever the other tiles hold, and the product of a tile is added in fp32 with
 // its factor; ref is only raised when a tile exceeds it by 2^40. Queries are scaled by the power of two that brings their
@@ -60,6 +60,7 @@ __device__ __forceinline__ int quant_len(const QuantAttnArgs& a, int i) {
 }
 
 constexpr int kTile = 16;   // tokens of a tile
+constexpr float kLowest = -3e38f;   // below every logit, and finite
 
 // Tiles of L tokens: none reaches over the end of a block.
 __device__ __forceinline__ int tiles_of(const QuantAttnArgs& a, int L) {
@@ -578,10 +579,14 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                         m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, x));
                         m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, x));
                     }
-                    m0 = fmaxf(fmaf(m0, f0, -15.f), -1e30f);   // a row that sees nothing of the tile: every weight 2^-inf
-                    m1 = fmaxf(fmaf(m1, f1, -15.f), -1e30f);
-                    const float p0 = ex2_fast(fmaf(s[n][0], f0, -m0)), p1 = ex2_fast(fmaf(s[n][1], f1, -m1));
-                    const float p2 = ex2_fast(fmaf(s[n][2], f0, -m0)), p3 = ex2_fast(fmaf(s[n][3], f1, -m1));
+                    m0 = fmaxf(m0, kLowest);   // a row that sees nothing of the tile: every weight 2^-inf
+                    m1 = fmaxf(m1, kLowest);
+                    // Differences of the sums first: the exponents end at 15 exactly. (2^(S f - m) against the rounded m = max f - 15 is
+                    // 2^16, infinite in fp16, from logits of 2^24 on.)
+                    const float p0 = ex2_fast(fmaf(s[n][0] - m0, f0, 15.f)), p1 = ex2_fast(fmaf(s[n][1] - m1, f1, 15.f));
+                    const float p2 = ex2_fast(fmaf(s[n][2] - m0, f0, 15.f)), p3 = ex2_fast(fmaf(s[n][3] - m1, f1, 15.f));
+                    m0 = fmaxf(m0 * f0, kLowest);
+                    m1 = fmaxf(m1 * f1, kLowest);
                     if (__any_sync(0xffffffffu, m0 > ref[n][0] + 40.f || m1 > ref[n][1] + 40.f)) {
                         const float u0 = fmaxf(ref[n][0], m0), u1 = fmaxf(ref[n][1], m1);
                         const float a0 = ex2_fast(ref[n][0] - u0), a1 = ex2_fast(ref[n][1] - u1);
@@ -824,7 +829,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps, U > 4 ? 1 : HD > 128 ? 3 : 4
     for (int e = 0; e < NV; ++e) v[e] = 0.f;
     float L = 0.f;
     if (here) {
-        float M = -1e30f;
+        float M = kLowest;
         for (int c = lane; c < parts; c += 32) M = fmaxf(M, ml[c * rows * 2]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));

@@ -1,0 +1,59 @@
+"""The 8-bit cache operators at the ends of their ranges: logits far beyond fp16, values near the largest fp32, scales that
+are no powers of two. Same oracle as the other tests of these operators."""
+import math
+
+import pytest
+import torch
+
+from oracle import quantized_cache as O
+from test_gpu_quantized_cache import DT, LENS, F, attention_inputs, bound_of, check_attention, check_copy, ctx, paged, take_status  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_status(F):  # noqa: F811
+    """No kernel of these tests meets anything that it has to report."""
+    assert take_status(F) is None
+    yield
+    assert take_status(F) is None
+
+
+# ---------------------------------------------------------------------------------------------------
+# logits
+# ---------------------------------------------------------------------------------------------------
+def small_integers(shape, e4m3, g):
+    """Codes of -3 .. 3."""
+    v = torch.randint(-3, 4, shape, generator=g)
+    return O.encode(v.double(), e4m3)
+
+
+@pytest.mark.parametrize("scale", [3e4, 1e5, 1e6, 1e9, 1e20, 1e27])
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("n,e4m3,bs,D", [(1, True, 16, 64), (3, True, 16, 128), (1, False, 24, 128), (3, False, 16, 256), (2, True, 16, 80)])
+def test_attention_of_huge_logits(F, ctx, n, e4m3, bs, D, dt, scale):  # noqa: F811
+    """Queries and keys of small integers, key scales of powers of two: every q . k * ks is a small multiple of 1/4, exact in
+    fp32, and logits of different ones are at least scale / 4 > 2^12 apart. So the weights are 1 / (number of tokens that share
+    the largest), 0 for the others, however the logits are rounded (by 2^-20 of themselves at most, and the largest is below
+    9 * D * 2 * 2^2 / 4 < 2^15 of those steps; equal products are rounded alike, as they only differ by powers of two in
+    their factors). What is left is the sum over equal weights (exact), one rounding of the quotient and of the value times
+    its scale, and the result's own."""
+    g = torch.Generator().manual_seed(n * 100 + D)
+    lens = LENS + [90, 400]
+    q, kc, vc, ks, vs, table, lens_t = attention_inputs(lens, n=n, e4m3=e4m3, bs=bs, D=D, dt=dt, seed=D + n)
+    q = torch.randint(-3, 4, q.shape, generator=g).to(DT[dt])
+    kc = small_integers(kc.shape, e4m3, g)
+    ks = 2.0 ** torch.randint(-2, 1, ks.shape, generator=g)
+    for sign in (1, -1):   # -1: every logit of some rows is far below zero
+        kk = kc
+        if sign < 0:
+            kk = small_integers(kc.shape, e4m3, g)
+            kk = O.encode(-O.decode(kk).abs() - 1, e4m3)
+        qq = q if sign > 0 else (q.abs() + 1)
+        want, (weight, _, _) = O.quantized_paged_attention(qq, kk, vc, ks, vs, table, lens_t, scale)
+        got = F.quantized_paged_attention(qq.cuda(), kk.cuda(), vc.cuda(), ks.cuda(), vs.cuda(), table.cuda(), lens_t.cuda(), scale, ctx=ctx).cpu().double()
+        ctx.release()
+        tiny = 2.0 ** -25 if dt == "fp16" else 1e-38
+        bound = weight * 2.0 ** -18 + want.abs() * torch.finfo(DT[dt]).eps / 2 + tiny
+        ok = (got - want).abs() <= bound
+        assert bool(ok.all()), f"{int((~ok).sum())} of {ok.numel()} values off, {int((~torch.isfinite(got)).sum())} not finite, first {(~ok).nonzero()[0].tolist()}"
