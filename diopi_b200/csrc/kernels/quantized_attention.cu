@@ -10,9 +10,9 @@
 //     S^T = Kc Q^T;  m = f max(S), f = ks * softmax_scale * log2 e;  P = 2^((S - max S) f + 15);  O^T += (2^(m - ref) vs) (Vc^T P^T)
 // The weights are taken against the tile's own maximum, so that they fill fp16's range (2^15 down to 2^-24: what is lost is
 // below 2^-40 of the tile's largest weight) whatever the other tiles hold, and the product of a tile is added in fp32 with
-// its factor; ref is only raised when a tile exceeds it by 2^40. Queries are scaled by the power of two that brings their
-// row's maximum to [1, 2) before they become fp16 (bf16 and fp32 reach further than fp16 does); fp32 queries and their
-// weights are split into two fp16 numbers each, with two products.
+// its factor; ref is only raised when a tile exceeds it by 2^16, or by less where values are above 2^41 (value_lift).
+// Queries are scaled by the power of two that brings their row's maximum to [1, 2) before they become fp16 (bf16 and fp32
+// reach further than fp16 does); fp32 queries and their weights are split into two fp16 numbers each, with two products.
 //
 // Work split: the tiles of the batch are cut into equal ranges, one per team, a team being the warps of one K/V head (one warp for up
 // to 8 * NT query rows, mt of them beyond). The teams of a CTA are hw neighbouring heads of the same range, which keeps their reads
@@ -62,6 +62,13 @@ __device__ __forceinline__ int quant_len(const QuantAttnArgs& a, int i) {
 constexpr int kTile = 16;   // tokens of a tile
 constexpr float kLowest = -3e38f;   // below every logit, and finite
 
+// How far the reference of the weights has to be above a logit in a block of value scale s, so that a sum of weights times values
+// stays finite wherever their mean is: s * 2^-lift < 2^(from + 1). 0 for the values that a model has.
+__device__ __forceinline__ float value_lift(float s, int from) { return static_cast<float>(max(static_cast<int>(__float_as_uint(s) << 1 >> 24) - 127 - from, 0)); }
+// What the reference of the split kernel may lag behind a tile's maximum. With a weight of 2^(15 + kLag - lift) at most the sum over
+// 2^31 tokens of code * s stays below 2^(31 + 9 + 42 + 31) = 2^113, and l above 2^(15 - 86).
+constexpr float kLag = 16.f;
+
 // Tiles of L tokens: none reaches over the end of a block.
 __device__ __forceinline__ int tiles_of(const QuantAttnArgs& a, int L) {
     if (a.block_size % kTile == 0) return (L + kTile - 1) / kTile;
@@ -110,7 +117,7 @@ __global__ void __launch_bounds__(32 * kPlainWarps) quant_plain_kernel(const Qua
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
         x *= ks;
-        const float mn = fmaxf(m, x);
+        const float mn = fmaxf(m, x + value_lift(vs, 64));   // a sum of 2^31 tokens ends below 2^(31 + 9 + 65)
         const float al = exp2f(m - mn), w = exp2f(x - mn);
         m = mn;
         l = fmaf(l, al, w);
@@ -561,6 +568,7 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                 }
                 uint32_t pb[NT][2], pl[NT][2];
                 float gain[NT][2];
+                const float lift = value_lift(vs, 41);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float f0 = ks * rs[n][0], f1 = ks * rs[n][1];
@@ -587,8 +595,9 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                     const float p2 = ex2_fast(fmaf(s[n][2] - m0, f0, 15.f)), p3 = ex2_fast(fmaf(s[n][3] - m1, f1, 15.f));
                     m0 = fmaxf(m0 * f0, kLowest);
                     m1 = fmaxf(m1 * f1, kLowest);
-                    if (__any_sync(0xffffffffu, m0 > ref[n][0] + 40.f || m1 > ref[n][1] + 40.f)) {
-                        const float u0 = fmaxf(ref[n][0], m0), u1 = fmaxf(ref[n][1], m1);
+                    const float r0 = m0 + lift, r1 = m1 + lift;
+                    if (__any_sync(0xffffffffu, r0 > ref[n][0] + kLag || r1 > ref[n][1] + kLag)) {
+                        const float u0 = fmaxf(ref[n][0], r0), u1 = fmaxf(ref[n][1], r1);
                         const float a0 = ex2_fast(ref[n][0] - u0), a1 = ex2_fast(ref[n][1] - u1);
                         ref[n][0] = u0;
                         ref[n][1] = u1;

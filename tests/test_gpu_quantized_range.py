@@ -57,3 +57,38 @@ def test_attention_of_huge_logits(F, ctx, n, e4m3, bs, D, dt, scale):  # noqa: F
         bound = weight * 2.0 ** -18 + want.abs() * torch.finfo(DT[dt]).eps / 2 + tiny
         ok = (got - want).abs() <= bound
         assert bool(ok.all()), f"{int((~ok).sum())} of {ok.numel()} values off, {int((~torch.isfinite(got)).sum())} not finite, first {(~ok).nonzero()[0].tolist()}"
+
+
+# ---------------------------------------------------------------------------------------------------
+# values
+# ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("factor", [1e18, 1e25, 1e32, 1e35, 1e-30])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,e4m3,D", [(1, True, 64), (1, False, 128), (3, True, 128), (2, True, 256), (2, True, 40)])
+def test_attention_of_huge_values(F, ctx, n, e4m3, D, dt, factor):  # noqa: F811
+    """Values that only the 8-bit exponent of bf16 and fp32 reaches, next to ordinary ones; logits that grow along the request,
+    so that the running maximum rises a little with almost every tile. The bounds are those of any other value: all of
+    them are relative to sum p |v|, but the one of the weights' last bits, which goes by the value itself (sum |v|)."""
+    lens = [1, 17, 40, 333, 700, 0]
+    q, kc, vc, ks, vs, table, lens_t = attention_inputs(lens, n=n, e4m3=e4m3, D=D, dt=dt, seed=D)
+    for i, L in enumerate(lens):
+        blocks = table[i, :-(-L // 16)]
+        ks[blocks] = 0.01 * torch.arange(1, len(blocks) + 1)[:, None] / 4
+    vs = vs.clamp(max=0.3) * factor / 3     # 448 * 0.1 * 1e35 < 3.4e38
+    check_attention(F, ctx, (q, kc, vc, ks, vs, table, lens_t))
+    ctx.release()
+    mixed = vs.clone()
+    mixed[::2] /= factor
+    check_attention(F, ctx, (q, kc, vc, ks, mixed, table, lens_t))
+    ctx.release()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,e4m3,D", [(1, True, 64), (3, True, 128), (1, False, 256), (2, False, 40)])
+def test_attention_where_the_sum_of_the_values_is_infinite(F, ctx, n, e4m3, D, dt):  # noqa: F811
+    """Equal weights over values just below the largest fp32: their mean is finite, their sum is not."""
+    lens = [1, 40, 700, 0]
+    q, kc, vc, ks, vs, table, lens_t = attention_inputs(lens, n=n, e4m3=e4m3, D=D, dt=dt, seed=D)
+    vc = vc & 0x7f if e4m3 else vc.abs()
+    vc = torch.where(vc == 0x7f, 0x7e, vc) if e4m3 else vc
+    check_attention(F, ctx, (torch.zeros_like(q), kc, vc.to(kc.dtype), ks, torch.full_like(vs, 3.2e38 / (448 if e4m3 else 127)), table, lens_t))
