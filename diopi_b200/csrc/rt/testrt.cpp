@@ -8,9 +8,12 @@
 // without a copy.
 //
 // Temporaries handed out through diopiRequireTensor/diopiRequireBuffer come from a
-// per-context cache of device blocks: a block is reused once the context has been
-// told (b200rt_context_release) that the work using it was enqueued; reuse is safe
-// because all work of a context goes to one stream.
+// per-context cache of blocks: a block is reused once the context has been told
+// (b200rt_context_release) that the work using it was enqueued, and only for work on
+// the stream that used it before, where that work comes first (another stream's might
+// still be reading it). Two exceptions: a stream that is being captured cannot allocate
+// and takes any free block (a block that a graph uses is that stream's from then on),
+// and when memory is out a block of another stream is taken after the device is idle.
 #include <cuda_runtime_api.h>
 
 #include <algorithm>
@@ -40,6 +43,7 @@ struct Block {
     int64_t bytes = 0;
     bool in_use = false;
     bool on_device = true;
+    cudaStream_t stream = nullptr;   // whose work used it last
 };
 
 int64_t elem_size(diopiDtype_t dt) {
@@ -137,27 +141,46 @@ RT_EXPORT diopiError_t diopiGetStream(diopiContextHandle_t ctx, diopiStreamHandl
     return diopiSuccess;
 }
 
+// The smallest free block that holds `bytes`, of the context's stream or of any.
+static Block* free_block(diopiContextHandle_t ctx, int64_t bytes, bool on_device, bool any_stream) {
+    Block* best = nullptr;
+    for (auto& b : ctx->blocks) {
+        if (b.in_use || b.on_device != on_device || b.bytes < bytes || (!any_stream && b.stream != ctx->stream)) continue;
+        if (!best || b.bytes < best->bytes) best = &b;
+    }
+    return best;
+}
+
+static bool capturing(cudaStream_t stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    return cudaStreamIsCapturing(stream, &status) == cudaSuccess && status == cudaStreamCaptureStatusActive;
+}
+
 static diopiError_t require_bytes(diopiContextHandle_t ctx, int64_t bytes, diopiDevice_t device, void** out) {
     ctx->n_require_calls++;
     const bool on_device = (device == diopi_device);
-    Block* best = nullptr;
-    for (auto& b : ctx->blocks) {
-        if (!b.in_use && b.on_device == on_device && b.bytes >= bytes && (!best || b.bytes < best->bytes)) best = &b;
-    }
+    Block* best = free_block(ctx, bytes, on_device, false);
+    if (!best && on_device && capturing(ctx->stream)) best = free_block(ctx, bytes, on_device, true);
     if (!best) {
         Block nb;
         nb.bytes = std::max<int64_t>(bytes, 256);
         nb.on_device = on_device;
-        if (on_device) {
-            if (cudaMalloc(&nb.ptr, nb.bytes) != cudaSuccess) return diopiErrorOccurred;
+        if (!on_device) {
+            nb.ptr = ::operator new(static_cast<size_t>(nb.bytes));
+        } else if (cudaMalloc(&nb.ptr, nb.bytes) == cudaSuccess) {
             ctx->n_device_allocs++;
         } else {
-            nb.ptr = ::operator new(static_cast<size_t>(nb.bytes));
+            cudaGetLastError();
+            best = free_block(ctx, bytes, on_device, true);
+            if (!best || cudaDeviceSynchronize() != cudaSuccess) return diopiErrorOccurred;
         }
-        ctx->blocks.push_back(nb);
-        best = &ctx->blocks.back();
+        if (!best) {
+            ctx->blocks.push_back(nb);
+            best = &ctx->blocks.back();
+        }
     }
     best->in_use = true;
+    best->stream = ctx->stream;
     *out = best->ptr;
     return diopiSuccess;
 }
@@ -270,7 +293,12 @@ RT_EXPORT diopiContextHandle_t b200rt_context_create(void* stream, int lazy) {
 
 RT_EXPORT void b200rt_context_set_stream(diopiContextHandle_t ctx, void* stream) {
     std::lock_guard<std::mutex> lock(ctx->mu);
-    if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
+    if (ctx->own_stream) {   // its blocks go on with the new stream
+        cudaStreamSynchronize(ctx->stream);
+        for (auto& b : ctx->blocks)
+            if (b.stream == ctx->stream) b.stream = static_cast<cudaStream_t>(stream);
+        cudaStreamDestroy(ctx->stream);
+    }
     ctx->own_stream = false;
     ctx->stream = static_cast<cudaStream_t>(stream);
     ctx->stream_ready = true;

@@ -115,7 +115,7 @@ class Context:
         self._stream = ptr
 
     def release(self) -> None:
-        """Lets the context reuse the scratch it handed out; call between steps."""
+        """Lets the context reuse the scratch it handed out, for work on the stream that used it; call between steps."""
         self._rt.b200rt_context_release(self.handle)
 
     def synchronize(self) -> None:
