@@ -8,6 +8,7 @@ a kernel) is handed to the C ABI by pointer, shape and stride, without a copy.
 from __future__ import annotations
 
 import ctypes
+import threading
 from ctypes import c_int64
 
 import torch
@@ -138,16 +139,19 @@ class Context:
             self._rt.b200rt_context_destroy(h)
 
 
-_default_ctx: dict[int, Context] = {}
+_default_ctx: dict[tuple[int, int], Context] = {}
 
 
 def default_context() -> Context:
-    """One context per CUDA device, on torch's current stream at the time of each call."""
+    """One context per thread and CUDA device, on torch's current stream at the time of each call. (Per thread: a call sets the
+    stream and then launches. A context outlives its thread, as a graph captured there may still use its scratch, and
+    serves the next thread of that identifier.)"""
     on_gpu = torch.cuda.is_initialized() or torch.cuda.is_available()   # the first is a look at a flag
     dev = torch.cuda.current_device() if on_gpu else -1
-    ctx = _default_ctx.get(dev)
+    key = (threading.get_ident(), dev)
+    ctx = _default_ctx.get(key)
     if ctx is None:
-        ctx = _default_ctx[dev] = Context()
+        ctx = _default_ctx[key] = Context()
     elif on_gpu:
         ptr = torch._C._cuda_getCurrentRawStream(dev)   # torch.cuda.current_stream() without the object around it
         if ptr != ctx._stream:

@@ -1,6 +1,7 @@
 """Scratch and streams of the contexts that the Python calls use. No GPU: host scratch stands for device scratch, and stream
 handles are numbers that nothing looks into."""
 import ctypes
+import threading
 from ctypes import byref, c_int64, c_void_p
 
 import pytest
@@ -57,6 +58,23 @@ def test_scratch_of_a_stream_is_used_again(rt, ctx):
         ctx.set_stream(0)
         assert scratch(rt, ctx) == first
     assert ctx.stats()["blocks"] == 1
+
+
+def test_each_thread_has_a_default_context(built_libs):
+    """A call sets the stream and then launches: between the two no other thread may set another one."""
+    from diopi_b200.runtime import default_context
+    mine, others, together = default_context(), [], threading.Barrier(3)
+
+    def work():
+        together.wait()      # all three alive at once: an identifier of a thread that has ended may come again
+        others.append(default_context())
+        together.wait()
+
+    ts = [threading.Thread(target=work) for _ in range(3)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert len({id(c) for c in (mine, *others)}) == 4
+    assert default_context() is mine
 
 
 @pytest.mark.gpu
