@@ -51,14 +51,15 @@ __device__ __forceinline__ int growth_steps(float old, float need) {
 __device__ __forceinline__ float pow2f(int k) { return k < -149 ? 0.f : exp2f(static_cast<float>(k)); }
 
 // One value, any input: the definition itself in double (a quotient of two fp32 values is never close enough to a tie of
-// an 8-bit format, without being one, for the double rounding to matter).
+// an 8-bit format, without being one, for the rounding to double to matter; a rounding to fp32 between the two would).
 template <bool E4M3>
 __device__ __noinline__ uint32_t encode_slow(float x, float s) {
     if (E4M3) {
         if (isnan(x)) return 0x7fu;
         if (s == 0.f) return 0u;
-        const float y = static_cast<float>(static_cast<double>(x) / static_cast<double>(s));   // s is a power of two
-        return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+        const double q = static_cast<double>(x) / static_cast<double>(s);
+        const float y = __double2float_rz(q);   // to odd: the code's rounding then sees all of q
+        return __nv_cvt_float_to_fp8(__uint_as_float(__float_as_uint(y) | (static_cast<double>(y) != q ? 1u : 0u)), __NV_SATFINITE, __NV_E4M3);
     }
     if (isnan(x) || s == 0.f) return 0u;
     double y = rint(static_cast<double>(x) / static_cast<double>(s));
@@ -72,7 +73,7 @@ __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
     return r;
 }
 
-// Four codes. e4m3: 1 / s is a power of two, so x * lo is exact (hi is not used). int8: adding 1.5 * 2^23 rounds x * inv to an
+// Four codes. e4m3: s is a power of two here, hence 1 / s, so x * lo is exact (hi is not used). int8: adding 1.5 * 2^23 rounds x * inv to an
 // integer, which sits in the low byte. `lo` and `hi` hold 1 / s between them (the approximate reciprocal is off by one unit
 // in the last place at most), so where both give one code the quotient has it; `split` collects the bits in which they differ.
 struct Inverse {
@@ -80,13 +81,15 @@ struct Inverse {
 };
 template <bool E4M3>
 __device__ __forceinline__ Inverse inverse_of(float s) {
-    const uint32_t u = __float_as_uint(s);
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
-    if (E4M3 && (u & 0x7fffffu) == 0) r = __uint_as_float(0x7f000000u - u);   // 2^-k of 2^k
     Inverse v;
-    v.lo = s > 0.f ? (E4M3 ? r : __uint_as_float(__float_as_uint(r) - 2)) : 0.f;
-    v.hi = s > 0.f ? (E4M3 ? r : __uint_as_float(__float_as_uint(r) + 2)) : 0.f;
+    if constexpr (E4M3) {
+        v.lo = v.hi = s > 0.f ? __uint_as_float(0x7f000000u - __float_as_uint(s)) : 0.f;   // 2^-k of 2^k
+    } else {
+        float r;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+        v.lo = s > 0.f ? __uint_as_float(__float_as_uint(r) - 2) : 0.f;
+        v.hi = s > 0.f ? __uint_as_float(__float_as_uint(r) + 2) : 0.f;
+    }
     return v;
 }
 constexpr float kMagic = 12582912.f;
@@ -223,7 +226,7 @@ constexpr int copy_ctas(int lpr) {
     return held <= 16 ? 4 : held <= 32 ? 3 : held <= 64 ? 2 : 1;
 }
 
-// One row of a unit with a NaN or an infinity in it; the lanes of a row share it.
+// One row of a unit that encode4 is not for (a NaN or an infinity in it, a scale of another kind); the lanes of a row share it.
 template <typename T, bool E4M3>
 __device__ __noinline__ void encode_row_slow(const T* x, uint8_t* to, int D, int first, int step, float s) {
     for (int d = first; d < D; d += step) to[d] = static_cast<uint8_t>(encode_slow<E4M3>(Cvt<T>::to_f(x[d]), s));
@@ -344,38 +347,42 @@ __global__ void __launch_bounds__(kCopyThreads, copy_ctas<T>(LPR)) quantized_cop
         }
         if (here && wu == 0 && lane == 0) *scale = s;
 
-        const Inverse inv = inverse_of<E4M3>(s);
-        for (int q = 0; q < chunks; ++q) {
-            if (REREAD) load_rows(q);
-            const int p = (q * W + wu) * kWarpRows + rl;
-            uint8_t* to = dst + p * a.c_s1[m] + cl * E;
+        // Of this file's own scales none: an e4m3 block that someone else began, with a scale that is no power of two.
+        const bool by_element = odd || (E4M3 && (__float_as_uint(s) & 0x7fffffu) != 0);
+        if (by_element) {   // the same for the whole unit; apart from the loop below, whose rows would be spilled around the call
+            for (int p = un.p0 + wu * RPP + rl; here && p < un.p1; p += W * RPP)
+                encode_row_slow<T, E4M3>(src + p * pitch, dst + p * a.c_s1[m], a.D, cl, LPR, s);
+        } else {
+            const Inverse inv = inverse_of<E4M3>(s);
+            for (int q = 0; q < chunks; ++q) {
+                if (REREAD) load_rows(q);
+                const int p = (q * W + wu) * kWarpRows + rl;
+                uint8_t* to = dst + p * a.c_s1[m] + cl * E;
 #pragma unroll
-            for (int i = 0; i < PASSES; ++i) {
-                const bool in = here && p + i * RPP >= un.p0 && p + i * RPP < un.p1;
-                if (in && odd) {
-                    encode_row_slow<T, E4M3>(src + (p + i * RPP) * pitch, to - cl * E, a.D, cl, LPR, s);
-                } else if (in) {
+                for (int i = 0; i < PASSES; ++i) {
+                    if (here && p + i * RPP >= un.p0 && p + i * RPP < un.p1) {
 #pragma unroll
-                    for (int n = 0; n < N; ++n) {
-                        if (!full_width && (n * LPR + cl) * E >= a.D) continue;
-                        float f[E];
-                        unpack16<T>(r[i][n], f);
-                        uint32_t w[E / 4], split = 0;
+                        for (int n = 0; n < N; ++n) {
+                            if (!full_width && (n * LPR + cl) * E >= a.D) continue;
+                            float f[E];
+                            unpack16<T>(r[i][n], f);
+                            uint32_t w[E / 4], split = 0;
 #pragma unroll
-                        for (int e = 0; e < E / 4; ++e) w[e] = encode4<E4M3>(f + 4 * e, inv, split);
-                        if (!E4M3 && split != 0) {
+                            for (int e = 0; e < E / 4; ++e) w[e] = encode4<E4M3>(f + 4 * e, inv, split);
+                            if (!E4M3 && split != 0) {
 #pragma unroll
-                            for (int e = 0; e < E / 4; ++e)
-                                w[e] = encode_near(f[4 * e], s, inv.lo) | (encode_near(f[4 * e + 1], s, inv.lo) << 8) | (encode_near(f[4 * e + 2], s, inv.lo) << 16) |
-                                       (encode_near(f[4 * e + 3], s, inv.lo) << 24);
+                                for (int e = 0; e < E / 4; ++e)
+                                    w[e] = encode_near(f[4 * e], s, inv.lo) | (encode_near(f[4 * e + 1], s, inv.lo) << 8) | (encode_near(f[4 * e + 2], s, inv.lo) << 16) |
+                                           (encode_near(f[4 * e + 3], s, inv.lo) << 24);
+                            }
+                            if constexpr (E == 8)
+                                *reinterpret_cast<uint2*>(to + n * LPR * E) = make_uint2(w[0], w[1]);
+                            else
+                                *reinterpret_cast<uint32_t*>(to + n * LPR * E) = w[0];
                         }
-                        if constexpr (E == 8)
-                            *reinterpret_cast<uint2*>(to + n * LPR * E) = make_uint2(w[0], w[1]);
-                        else
-                            *reinterpret_cast<uint32_t*>(to + n * LPR * E) = w[0];
                     }
+                    to += RPP * a.c_s1[m];
                 }
-                to += RPP * a.c_s1[m];
             }
         }
         if constexpr (W > 1) __syncthreads();   // s_top is written again

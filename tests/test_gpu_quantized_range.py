@@ -92,3 +92,63 @@ def test_attention_where_the_sum_of_the_values_is_infinite(F, ctx, n, e4m3, D, d
     vc = vc & 0x7f if e4m3 else vc.abs()
     vc = torch.where(vc == 0x7f, 0x7e, vc) if e4m3 else vc
     check_attention(F, ctx, (torch.zeros_like(q), kc, vc.to(kc.dtype), ks, torch.full_like(vs, 3.2e38 / (448 if e4m3 else 127)), table, lens_t))
+
+
+# ---------------------------------------------------------------------------------------------------
+# scales of the store
+# ---------------------------------------------------------------------------------------------------
+def store_both(F, ctx, x, table, cached, starts, cache, scale, wide):  # noqa: F811
+    """The store's codes and scales; `wide`: in a cache whose rows are one byte too far apart for the vector kernel."""
+    dc = []
+    for _ in range(2):
+        c = cache.cuda()
+        if wide:
+            big = torch.zeros(*cache.shape[:-1], cache.shape[-1] + 1, dtype=cache.dtype, device="cuda")
+            big[..., :-1] = c
+            c = big[..., :-1]
+        dc.append(c)
+    ds = [scale.cuda() for _ in range(2)]
+    F.quantized_copy_kv(x.cuda(), x.cuda(), table.cuda(), cached.cuda(), starts.cuda(), *dc, *ds, ctx=ctx)
+    return dc, ds
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("e4m3", [True, False])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_copy_into_blocks_of_any_scale(F, ctx, D, dt, e4m3, wide):  # noqa: F811
+    """Blocks that someone else began, with scales of any mantissa (amax / 448 for one): the new values sit on the borders
+    between two codes of the scale that the block has or grows to, and one step of their type beside them."""
+    g = torch.Generator().manual_seed(D)
+    B, H, bs = 24, 3, 16
+    table = torch.randperm(B + 2, generator=g)[:B, None]
+    cached = torch.randint(1, 8, (B,), generator=g)
+    new = torch.randint(1, 8, (B,), generator=g)
+    starts = torch.cat([torch.zeros(1, dtype=torch.int64), new.cumsum(0)])
+    scale = torch.rand(B + 2, H, generator=g) + 0.5
+    scale[::3] = torch.randint(65, 128, scale[::3].shape, generator=g) / 64.0       # ties that bf16 holds
+    scale *= 2.0 ** torch.randint(-20, 20, scale.shape, generator=g)
+    grow = torch.randint(0, 4, (B, H), generator=g)
+    who = torch.repeat_interleave(torch.arange(B), new)
+    s = scale[table[who, 0]].double() * 2.0 ** grow[who]          # the scale that each block ends with
+    # The value that makes it grow to that: a fresh block's scale for it is above s / 2 and not above s.
+    top = 448.0 * 2.0 ** torch.floor(torch.log2(s)) if e4m3 else 127.0 * 0.75 * s
+    v = O.e4m3_values()[:127] if e4m3 else torch.arange(0, 96, dtype=torch.float64)
+    border = (v[:-1] + v[1:]) / 2
+    border = border[border < (220 if e4m3 else 95)]
+    T = int(new.sum())
+    pick = border[torch.randint(0, len(border), (T, H, D), generator=g)] * (1 - 2.0 * torch.randint(0, 2, (T, H, D), generator=g))
+    pick = pick * s[:, :, None]
+    pick[:, :, 0] = top
+    x = pick.to(DT[dt])
+    eps = torch.finfo(DT[dt]).eps
+    beside = torch.randint(-1, 2, (T, H, D), generator=g)
+    beside[:, :, 0] = 0
+    x = torch.where(beside == 0, x, (x.double() * (1 + eps * beside)).to(DT[dt]))
+    cache = torch.randint(0, 120, (B + 2, bs, H, D), generator=g).to(torch.uint8 if e4m3 else torch.int8)
+    want = O.quantized_copy(x, table, cached, starts, cache, scale)
+    dc, ds = store_both(F, ctx, x, table, cached, starts, cache, scale, wide)
+    for m in range(2):
+        assert torch.equal(ds[m].cpu(), want[1])
+        diff = dc[m].cpu() != want[0]
+        assert not bool(diff.any()), f"{int(diff.sum())} of {T * H * D} codes differ, first at {diff.nonzero()[0].tolist()}"
