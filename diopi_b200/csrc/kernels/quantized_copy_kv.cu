@@ -347,8 +347,9 @@ __global__ void __launch_bounds__(kCopyThreads, copy_ctas<T>(LPR)) quantized_cop
         }
         if (here && wu == 0 && lane == 0) *scale = s;
 
-        // Of this file's own scales none: an e4m3 block that someone else began, with a scale that is no power of two.
-        const bool by_element = odd || (E4M3 && (__float_as_uint(s) & 0x7fffffu) != 0);
+        // Of this file's own scales none: a block that someone else began, with a scale that has no reciprocal among the normal numbers, or
+        // that is no power of two where the codes are e4m3.
+        const bool by_element = odd || s > 0x1p126f || (E4M3 && (__float_as_uint(s) & 0x7fffffu) != 0);
         if (by_element) {   // the same for the whole unit; apart from the loop below, whose rows would be spilled around the call
             for (int p = un.p0 + wu * RPP + rl; here && p < un.p1; p += W * RPP)
                 encode_row_slow<T, E4M3>(src + p * pitch, dst + p * a.c_s1[m], a.D, cl, LPR, s);

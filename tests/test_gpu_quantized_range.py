@@ -152,3 +152,22 @@ def test_copy_into_blocks_of_any_scale(F, ctx, D, dt, e4m3, wide):  # noqa: F811
         assert torch.equal(ds[m].cpu(), want[1])
         diff = dc[m].cpu() != want[0]
         assert not bool(diff.any()), f"{int(diff.sum())} of {T * H * D} codes differ, first at {diff.nonzero()[0].tolist()}"
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("e4m3", [True, False])
+def test_copy_into_blocks_of_the_largest_scales(F, ctx, e4m3, wide):  # noqa: F811
+    """Scales whose reciprocal is no normal fp32 number, and subnormal ones."""
+    g = torch.Generator().manual_seed(1)
+    scale = torch.tensor([[2.0 ** 125, 2.0 ** 126], [2.0 ** 127, 1.5 * 2.0 ** 126], [1.9 * 2.0 ** 127, 2.0 ** -127], [2.0 ** -140, 2.0 ** -126]])
+    x = (torch.randn(8, 2, 64, generator=g) * 2.0 ** 125).float()
+    x[6:, 0] *= 0.0
+    x[4:6, 1] *= 2.0 ** -251
+    x[6:, 1] *= 2.0 ** -251
+    table, cached, starts = torch.arange(4)[:, None], torch.full((4,), 5), torch.arange(0, 9, 2)
+    cache = torch.randint(0, 120, (4, 16, 2, 64), generator=g).to(torch.uint8 if e4m3 else torch.int8)
+    want = O.quantized_copy(x, table, cached, starts, cache, scale)
+    dc, ds = store_both(F, ctx, x, table, cached, starts, cache, scale, wide)
+    for m in range(2):
+        assert torch.equal(ds[m].cpu(), want[1])
+        assert torch.equal(dc[m].cpu(), want[0])
