@@ -355,6 +355,7 @@ __global__ void __launch_bounds__(kCopyThreads, copy_ctas<T>(LPR)) quantized_cop
                 encode_row_slow<T, E4M3>(src + p * pitch, dst + p * a.c_s1[m], a.D, cl, LPR, s);
         } else {
             const Inverse inv = inverse_of<E4M3>(s);
+            const uint32_t nonzero = E4M3 && s == 0.f ? 0u : 0xffffffffu;   // a block of zeros has codes 0: no -0 (0x80) for a -0
             for (int q = 0; q < chunks; ++q) {
                 if (REREAD) load_rows(q);
                 const int p = (q * W + wu) * kWarpRows + rl;
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(kCopyThreads, copy_ctas<T>(LPR)) quantized_cop
                             unpack16<T>(r[i][n], f);
                             uint32_t w[E / 4], split = 0;
 #pragma unroll
-                            for (int e = 0; e < E / 4; ++e) w[e] = encode4<E4M3>(f + 4 * e, inv, split);
+                            for (int e = 0; e < E / 4; ++e) w[e] = encode4<E4M3>(f + 4 * e, inv, split) & nonzero;
                             if (!E4M3 && split != 0) {
 #pragma unroll
                                 for (int e = 0; e < E / 4; ++e)

@@ -171,3 +171,22 @@ def test_copy_into_blocks_of_the_largest_scales(F, ctx, e4m3, wide):  # noqa: F8
     for m in range(2):
         assert torch.equal(ds[m].cpu(), want[1])
         assert torch.equal(dc[m].cpu(), want[0])
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("e4m3", [True, False])
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_copy_of_zeros_of_both_signs(F, ctx, dt, e4m3, wide):  # noqa: F811
+    """A block of nothing but zeros has scale 0 and codes 0, whatever their signs; in a block with a scale a negative zero keeps its sign."""
+    g = torch.Generator().manual_seed(4)
+    x = torch.zeros(40, 2, 64)
+    x[torch.rand(x.shape, generator=g) < 0.5] = -0.0
+    x[20:, 1, 5] = 3.0
+    x = x.to(DT[dt])
+    table, cached, starts = torch.tensor([[0, 1], [2, 3]]), torch.tensor([0, 9]), torch.tensor([0, 20, 40])
+    cache, scale = torch.zeros(5, 16, 2, 64, dtype=torch.uint8 if e4m3 else torch.int8), torch.zeros(5, 2)
+    want = O.quantized_copy(x, table, cached, starts, cache, scale)
+    dc, ds = store_both(F, ctx, x, table, cached, starts, cache, scale, wide)
+    assert bool((want[0][:2] == 0).all()) and (not e4m3 or bool((want[0][2:4, :, 1] == 0x80).any()))
+    for m in range(2):
+        assert torch.equal(dc[m].cpu(), want[0]) and torch.equal(ds[m].cpu(), want[1])
