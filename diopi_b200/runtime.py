@@ -39,8 +39,9 @@ _TORCH_TO_DIOPI = {
     torch.int8: Dtype.int8, torch.uint8: Dtype.uint8, torch.int16: Dtype.int16, torch.int32: Dtype.int32,
     torch.int64: Dtype.int64, torch.float16: Dtype.float16, torch.float32: Dtype.float32,
     torch.float64: Dtype.float64, torch.bool: Dtype.bool, torch.bfloat16: Dtype.bfloat16,
-    torch.float8_e4m3fn: Dtype.uint8,   # the interface has no 8-bit float: ops that take e4m3 take its bits as uint8
 }
+# The interface has no 8-bit float: the ops on 8-bit caches take the bits of e4m3 codes as uint8. Only theirs.
+_CODES_TO_DIOPI = {**_TORCH_TO_DIOPI, torch.float8_e4m3fn: Dtype.uint8}
 
 SUCCESS, ERROR_OCCURRED, NO_IMPLEMENT, DTYPE_NOT_SUPPORTED = 0, 1, 13, 1000
 
@@ -80,14 +81,14 @@ _pycall = None
 
 
 def call_with(op: str, ctx_handle, tensors: tuple, extra=None, as_device: bool | None = None) -> int:
-    """The return code of op(ctx, handles of `tensors`..., extra), with handles that live as long as the call. Each item is
-    a torch tensor, a Tensor or None; `extra` an int (int64_t), a float (double) or None. Tensors of another device than
+    """The return code of op(ctx, handles of `tensors`..., extra), an op on 8-bit caches, with handles that live as long as the call.
+    Each item is a torch tensor, a Tensor or None; `extra` an int (int64_t), a float (double) or None. Tensors of another device than
     the current one are refused: the op would be launched beside its own memory."""
     global _pycall
     if _pycall is None:
         libs = _lib.load()
         address = lambda fn: ctypes.cast(fn, ctypes.c_void_p).value  # noqa: E731
-        libs.pycall.init(address(libs.rt.b200rt_batch_create), address(libs.rt.b200rt_batch_destroy), _TORCH_TO_DIOPI, Tensor)
+        libs.pycall.init(address(libs.rt.b200rt_batch_create), address(libs.rt.b200rt_batch_destroy), _CODES_TO_DIOPI, Tensor)
         _pycall = libs.pycall.call
     current = torch.cuda.current_device() if as_device is None and torch.cuda.is_initialized() else -1
     return _pycall(_lib._libs.address[op], ctx_handle, tensors, extra, as_device, current)
