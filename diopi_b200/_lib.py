@@ -11,6 +11,7 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import os
+import sysconfig
 from ctypes import POINTER, c_bool, c_char_p, c_double, c_int, c_int64, c_void_p
 from pathlib import Path
 
@@ -26,7 +27,6 @@ class diopiSize_t(ctypes.Structure):
 class _Libs:
     rt: ctypes.CDLL | None = None
     impl: ctypes.CDLL | None = None
-    pycall = None          # the module that calls an op with torch tensors; see runtime.call_with
     address: dict = {}     # op name -> address
 
 
@@ -72,8 +72,7 @@ def load() -> _Libs:
         return _libs
     rt_path = LIB_DIR / "libdiopi_rt.so"
     impl_path = LIB_DIR / "libdiopi_impl.so"
-    py_path = LIB_DIR / "_pycall.so"
-    for p in (rt_path, impl_path, py_path):
+    for p in (rt_path, impl_path):
         if not p.exists():
             raise RuntimeError(
                 f"{p} is missing: the CUDA libraries of diopi_b200 are not built "
@@ -111,9 +110,22 @@ def load() -> _Libs:
         fn = getattr(impl, name)
         fn.restype = c_char_p
         fn.argtypes = []
-    loader = importlib.machinery.ExtensionFileLoader("_pycall", str(py_path))
-    pycall = importlib.util.module_from_spec(importlib.util.spec_from_loader("_pycall", loader))
-    loader.exec_module(pycall)
     _libs.address = {name: ctypes.cast(getattr(impl, name), c_void_p).value for name in OPS}
-    _libs.rt, _libs.impl, _libs.pycall = rt, impl, pycall
+    _libs.rt, _libs.impl = rt, impl
     return _libs
+
+
+def pycall_name() -> str:
+    """The file of the call module for the running Python; another one's has another name."""
+    return "_pycall" + sysconfig.get_config_var("EXT_SUFFIX")
+
+
+def load_pycall():
+    """The CPython module that calls an op with torch tensors (runtime.call_with), loaded at the first such call."""
+    path = LIB_DIR / pycall_name()
+    if not path.exists():
+        raise RuntimeError(f"{path} is missing: run `python -m diopi_b200.build` with this Python (it needs the Python headers)")
+    loader = importlib.machinery.ExtensionFileLoader("_pycall", str(path))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_pycall", loader))
+    loader.exec_module(module)
+    return module

@@ -88,8 +88,9 @@ def call_with(op: str, ctx_handle, tensors: tuple, extra=None, as_device: bool |
     if _pycall is None:
         libs = _lib.load()
         address = lambda fn: ctypes.cast(fn, ctypes.c_void_p).value  # noqa: E731
-        libs.pycall.init(address(libs.rt.b200rt_batch_create), address(libs.rt.b200rt_batch_destroy), _CODES_TO_DIOPI, Tensor)
-        _pycall = libs.pycall.call
+        pycall = _lib.load_pycall()
+        pycall.init(address(libs.rt.b200rt_batch_create), address(libs.rt.b200rt_batch_destroy), _CODES_TO_DIOPI, Tensor)
+        _pycall = pycall.call
     current = torch.cuda.current_device() if as_device is None and torch.cuda.is_initialized() else -1
     return _pycall(_lib._libs.address[op], ctx_handle, tensors, extra, as_device, current)
 
