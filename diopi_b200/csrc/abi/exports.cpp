@@ -5,6 +5,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <numeric>
 #include <unordered_map>
 
 #include "../kernels/kernels.hpp"
@@ -1000,12 +1001,41 @@ void byte_range(const TensorView& t, uintptr_t& lo, uintptr_t& hi) {
     hi += static_cast<uintptr_t>(e);
 }
 
+// The bytes of a view as runs: `run` bytes without a gap, at multiples of `step` (0: one run) behind the first.
+void runs_of(const TensorView& t, int64_t& run, int64_t& step) {
+    const int64_t e = t.elem_size();
+    int64_t stride[kMaxDims], extent[kMaxDims];
+    int n = 0;
+    for (int i = 0; i < t.ndim; ++i) {
+        if (t.shape[i] <= 1 || t.stride[i] == 0) continue;
+        const int64_t s = std::abs(t.stride[i]) * e;
+        int at = n++;
+        for (; at > 0 && stride[at - 1] > s; --at) stride[at] = stride[at - 1], extent[at] = extent[at - 1];
+        stride[at] = s;
+        extent[at] = t.shape[i];
+    }
+    run = e;
+    step = 0;
+    int i = 0;
+    for (; i < n && stride[i] == run; ++i) run *= extent[i];
+    for (; i < n; ++i) step = std::gcd(step, stride[i]);
+}
+
+// Whether two views share memory. Views whose runs alternate (slices of a fused tensor) do not: modulo the steps' common divisor
+// each touches one window only. Others whose ranges overlap are taken to share.
 bool overlap(const TensorView& a, const TensorView& b) {
     if (!a.defined || !b.defined || a.numel == 0 || b.numel == 0) return false;
     uintptr_t al, ah, bl, bh;
     byte_range(a, al, ah);
     byte_range(b, bl, bh);
-    return al < bh && bl < ah;
+    if (al >= bh || bl >= ah) return false;
+    int64_t ra, rb, sa, sb;
+    runs_of(a, ra, sa);
+    runs_of(b, rb, sb);
+    const int64_t g = std::gcd(sa, sb);
+    if (g == 0 || ra + rb > g) return true;
+    const int64_t ahead = static_cast<int64_t>((bl % g + g - al % g) % g);   // of b's window before the next of a's
+    return ahead < ra || g - ahead < rb;
 }
 
 // Elements of a tensor that a kernel writes must not share memory: an expanded dim would make rows of it one.

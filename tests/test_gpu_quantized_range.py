@@ -190,3 +190,26 @@ def test_copy_of_zeros_of_both_signs(F, ctx, dt, e4m3, wide):  # noqa: F811
     assert bool((want[0][:2] == 0).all()) and (not e4m3 or bool((want[0][2:4, :, 1] == 0x80).any()))
     for m in range(2):
         assert torch.equal(dc[m].cpu(), want[0]) and torch.equal(ds[m].cpu(), want[1])
+
+
+# ---------------------------------------------------------------------------------------------------
+# views
+# ---------------------------------------------------------------------------------------------------
+def test_slices_of_one_fused_tensor(F, ctx):  # noqa: F811
+    """q and out are slices of one projection; lengths, offsets and slots are columns of one tensor."""
+    args = attention_inputs(LENS, D=64, n=2)
+    fused = torch.full((len(LENS), 2, 3, 8, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    views = {"q": fused[:, :, 0], "out": fused[:, :, 2]}
+    check_attention(F, ctx, args, view=lambda kind, t: views[kind].copy_(t) if kind in views else t)
+    assert bool((fused[:, :, 1] == 7).all()) and torch.equal(fused[:, :, 0].cpu(), args[0])
+    i32 = dict(dtype=torch.int32, device="cuda")
+    t = torch.full((8, 5), -3, **i32)
+    t[:3, 0], t[:3, 1] = torch.tensor([4, 0, 9], **i32), torch.tensor([1, 5, 2], **i32)
+    table = torch.full((3, 4), -1, **i32)
+    table[0, 0], table[2, :3] = 0, torch.tensor([1, 2, 3], **i32)
+    F.build_block_table(table, t[:3, 0], t[:3, 1], torch.arange(20, 0, -1, **i32), torch.zeros(1, **i32), 4, slot_map=t[:, 2], new_start=t[:4, 3], seq_lens=t[:3, 4],
+                        free_next=torch.zeros(1, **i32), ctx=ctx)
+    assert t[:, 0].tolist() == [4, 0, 9] + [-3] * 5 and t[:, 1].tolist() == [1, 5, 2] + [-3] * 5
+    assert t[:, 3].tolist() == [0, 1, 6, 8] + [-3] * 4 and t[:, 4].tolist() == [5, 5, 11] + [-3] * 5
+    # blocks taken: 20 | 19, 18 | none
+    assert t[:, 2].tolist() == [80, 76, 77, 78, 79, 72, 13, 14]

@@ -184,3 +184,42 @@ def test_what_a_call_takes(F, built_libs):
     with pytest.raises(AttributeError):
         F.quantized_copy_kv(*{**cache_args(), "k": [1, 2]}.values(), as_device=True)
     fails(ERROR_OCCURRED, F.quantized_copy_kv, *{**cache_args(), "k": torch.zeros([1] * 9)}.values(), match="at most 8")
+
+
+# ---- views that interleave ---------------------------------------------------------------------------
+def test_views_that_alternate_do_not_share_memory(F):
+    """Slices of one fused tensor whose byte ranges overlap but whose elements do not are no overlap: what is refused in these calls
+    is a later argument. Slices that do share elements are refused as such."""
+    c = cache_args()
+    fused = torch.zeros(2, 3, 8, 32, dtype=torch.float16)
+    cols = torch.zeros(2, 8, 64, dtype=torch.float16)
+
+    def attend(q, out, match):
+        fails(ERROR_OCCURRED, F.quantized_paged_attention, q, c["k_cache"], c["v_cache"], c["k_scale"], c["v_scale"], c["block_table"], c["cached_lens"], -1.0,
+              match=match, out=out)
+
+    attend(fused[:, 0], fused[:, 2], "softmax_scale")
+    attend(fused[:, 1], fused[:, 0], "softmax_scale")
+    attend(cols[..., :32], cols[..., 32:], "softmax_scale")
+    attend(cols[..., :32], cols[..., 16:48], "not overlap")
+    attend(fused[:, 0], fused.view(2, 24, 32)[:, 4:12], "not overlap")
+    attend(fused.view(6, 8, 32)[:2], fused.view(6, 8, 32)[1:3], "not overlap")
+    # the same with the head dim's rows apart: heads in front of the batch
+    heads = torch.zeros(8, 2, 2, 32, dtype=torch.float16)
+    attend(heads[:, 0].transpose(0, 1), heads[:, 1].transpose(0, 1), "softmax_scale")
+
+    i32 = dict(dtype=torch.int32)
+    both, five = torch.zeros(2, 2, **i32), torch.zeros(3, 5, **i32)
+
+    def tables(match, **over):
+        a, kw = table_args()
+        a["block_size"] = 1 << 29      # refused after the views have been looked at
+        for k, v in over.items():
+            (a if k in a else kw)[k] = v
+        fails(ERROR_OCCURRED, F.build_block_table, *a.values(), match=match, **kw)
+
+    tables("2\\^31", cached_lens=both[:, 0], seq_lens=both[:, 1])
+    tables("2\\^31", new_start=five[:, 0], seq_lens=five[:2, 2], new_lens=five[:2, 4], slot_map=five[:, 1])
+    tables("share memory", cached_lens=both[:, 0], seq_lens=both[:, 0])
+    tables("share memory", new_start=five[:, 0], seq_lens=five[:2, 0])
+    tables("share memory", slot_map=both.view(-1), seq_lens=both[:, 1])
