@@ -421,7 +421,16 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float scale = 1.f, back = 1.f;
-                if constexpr (!std::is_same<T, __half>::value) {   // 2^-e with the row's maximum in [2^e, 2^(e + 1))
+                bool infinite;   // logits of this row can only be infinite or NaN, so its result is NaN: also where all of them are -inf
+                if constexpr (std::is_same<T, __half>::value) {
+                    __half2 top = __float2half2_rn(0.f);
+#pragma unroll
+                    for (int i = 0; i < CH; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) top = __hmax2(top, __habs2(*reinterpret_cast<const __half2*>(&qf[n][i][h])));
+                    const uint32_t lanes = __ballot_sync(0xffffffffu, __half2float(__hmax(top.x, top.y)) == INFINITY);
+                    infinite = (lanes >> (lane & 28) & 15u) != 0;
+                } else {   // 2^-e with the row's maximum in [2^e, 2^(e + 1))
                     float amax = 0.f;
 #pragma unroll
                     for (int i = 0; i < CH; ++i)
@@ -435,6 +444,7 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                         }
                     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                    infinite = amax == INFINITY;
                     const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
                     scale = __uint_as_float((254u - e) << 23);
                     back = __uint_as_float(e << 23);
@@ -454,7 +464,7 @@ __global__ void __launch_bounds__(32 * split_warps(std::is_same<T, float>::value
                         }
                     }
                 }
-                back *= a.softmax_scale * kLog2e;
+                back = infinite ? __int_as_float(0x7fffffff) : back * (a.softmax_scale * kLog2e);
                 rs[n][0] = __shfl_sync(0xffffffffu, back, 8 * c);       // of row 2c
                 rs[n][1] = __shfl_sync(0xffffffffu, back, 8 * c + 4);   // of row 2c + 1
 #pragma unroll

@@ -213,3 +213,24 @@ def test_slices_of_one_fused_tensor(F, ctx):  # noqa: F811
     assert t[:, 3].tolist() == [0, 1, 6, 8] + [-3] * 4 and t[:, 4].tolist() == [5, 5, 11] + [-3] * 5
     # blocks taken: 20 | 19, 18 | none
     assert t[:, 2].tolist() == [80, 76, 77, 78, 79, 72, 13, 14]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("n,e4m3,D", [(1, True, 64), (3, True, 128), (2, False, 256), (1, False, 40)])
+def test_attention_of_infinite_queries(F, ctx, n, e4m3, D, dt):  # noqa: F811
+    """An infinity in a row of q makes every logit of that row infinite or NaN, hence the row NaN, also where all of them are -inf;
+    rows that see no token stay zeros, and no other row is touched."""
+    lens = [0, 1, 40, 16, 700, 300]
+    q, kc, vc, ks, vs, table, lens_t = attention_inputs(lens, n=n, e4m3=e4m3, D=D, dt=dt, seed=D)
+    kc[..., 5] = 0x30 if e4m3 else 17          # every key is positive here
+    clean = q.clone()
+    bad = torch.zeros(q.shape[:3], dtype=torch.bool)
+    for i, (t, h, x) in enumerate(((0, 0, -math.inf), (n - 1, 1, -math.inf), (0, 2, math.inf), (n - 1, 3, -math.inf), (n - 1, 7, -math.inf), (0, 4, math.inf))):
+        q[i, t, h, 5] = x
+        clean[i, t, h, 5] = 0
+        bad[i, t, h] = lens[i] - (n - 1 - t) > 0
+    got = F.quantized_paged_attention(q.cuda(), kc.cuda(), vc.cuda(), ks.cuda(), vs.cuda(), table.cuda(), lens_t.cuda(), 0.1, ctx=ctx).cpu()
+    assert torch.equal(torch.isnan(got), bad[..., None].expand_as(got))
+    want, sums = O.quantized_paged_attention(clean, kc, vc, ks, vs, table, lens_t, 0.1)
+    ok = (got.double() - want).abs() <= bound_of(want, sums, 700, D, q.dtype)
+    assert bool((ok | bad[..., None]).all())
