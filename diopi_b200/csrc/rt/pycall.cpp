@@ -135,9 +135,10 @@ PyObject* call(PyObject*, PyObject* const* a, Py_ssize_t na) {
         whole = PyLong_AsLongLong(a[3]);
     if (PyErr_Occurred()) return nullptr;
     int rc;
-    Py_BEGIN_ALLOW_THREADS;
     void* h[kMaxTensors];
     void* batch = g.create(desc, static_cast<int>(n), h);
+    if (!batch) return PyErr_NoMemory();
+    Py_BEGIN_ALLOW_THREADS;
     for (Py_ssize_t i = 0; i < n; ++i)
         if (given[i]) h[i] = given[i];
     if (is_real)

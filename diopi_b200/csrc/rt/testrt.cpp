@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <cstdio>
 #include <cstring>
+#include <memory>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -256,9 +257,10 @@ RT_EXPORT void b200rt_tensor_destroy(diopiTensorHandle_t t) { delete t; }
 
 // The handles of one call at once (a call into this library per tensor is what a Python caller spends most of its time on).
 // `desc` holds, one tensor after the other, ndim, dtype, device, data pointer, shape[ndim], stride[ndim]; ndim = -1 alone
-// stands for a null handle. The handles go to `out`; the returned batch is what b200rt_batch_destroy takes.
-RT_EXPORT void* b200rt_batch_create(const int64_t* desc, int n, void** out) {
-    auto* batch = new std::vector<diopiTensor>(static_cast<size_t>(n));
+// stands for a null handle. The handles go to `out`; the returned batch is what b200rt_batch_destroy
+// takes; null: no memory for them.
+RT_EXPORT void* b200rt_batch_create(const int64_t* desc, int n, void** out) try {
+    auto batch = std::make_unique<std::vector<diopiTensor>>(static_cast<size_t>(n));
     for (int i = 0; i < n; ++i) {
         const int64_t nd = *desc++;
         out[i] = nullptr;
@@ -275,7 +277,9 @@ RT_EXPORT void* b200rt_batch_create(const int64_t* desc, int n, void** out) {
         for (auto s : t.shape) t.numel *= s;
         out[i] = &t;
     }
-    return batch;
+    return batch.release();
+} catch (...) {
+    return nullptr;
 }
 
 RT_EXPORT void b200rt_batch_destroy(void* batch) { delete static_cast<std::vector<diopiTensor>*>(batch); }

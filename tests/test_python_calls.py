@@ -96,3 +96,20 @@ def test_build_without_python_headers(monkeypatch, tmp_path, capsys):
     assert set(build()) == {"impl", "rt"} and "Python.h" in capsys.readouterr().err
     build()
     assert build.linked == []
+
+
+def test_handles_that_cannot_be_made_are_an_error(built_libs):
+    """A C entry of the run time gives null back; an exception that leaves it would end the process (hence one of its own here)."""
+    import subprocess
+    import sys
+    from diopi_b200 import _lib
+    code = """
+import ctypes
+from diopi_b200 import _lib
+rt = _lib.load().rt
+rt.b200rt_batch_create.restype = ctypes.c_void_p
+rt.b200rt_batch_create.argtypes = [ctypes.POINTER(ctypes.c_int64), ctypes.c_int, ctypes.c_void_p]
+print(rt.b200rt_batch_create((ctypes.c_int64 * 4)(), -1, None))
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=_lib.LIB_DIR.parent.parent)
+    assert r.returncode == 0 and r.stdout.strip() == "None", (r.returncode, r.stderr[-300:])
