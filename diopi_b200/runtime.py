@@ -141,7 +141,22 @@ class Context:
             self._rt.b200rt_context_destroy(h)
 
 
-_default_ctx: dict[tuple[int, int], Context] = {}
+class _DefaultContext(Context):
+    """The context of a thread's calls on a device that name none. A release is for the device: the contexts of other threads, which
+    may be in a call, take it up with their next one (a backward pass runs on a thread that has nobody to release for it)."""
+
+    def __init__(self, device: int):
+        super().__init__()
+        self.device, self.release_due = device, False
+
+    def release(self) -> None:
+        super().release()
+        for other in list(_default_ctx.values()):
+            if other is not self and other.device == self.device:
+                other.release_due = True
+
+
+_default_ctx: dict[tuple[int, int], _DefaultContext] = {}
 
 
 def default_context() -> Context:
@@ -153,11 +168,14 @@ def default_context() -> Context:
     key = (threading.get_ident(), dev)
     ctx = _default_ctx.get(key)
     if ctx is None:
-        ctx = _default_ctx[key] = Context()
+        ctx = _default_ctx[key] = _DefaultContext(dev)
     elif on_gpu:
         ptr = torch._C._cuda_getCurrentRawStream(dev)   # torch.cuda.current_stream() without the object around it
         if ptr != ctx._stream:
             ctx.set_stream(ptr)
+    if ctx.release_due:
+        ctx.release_due = False
+        Context.release(ctx)
     return ctx
 
 

@@ -1,6 +1,7 @@
 """Scratch and streams of the contexts that the Python calls use. No GPU: host scratch stands for device scratch, and stream
 handles are numbers that nothing looks into."""
 import ctypes
+import queue
 import threading
 from ctypes import byref, c_int64, c_void_p
 
@@ -75,6 +76,36 @@ def test_each_thread_has_a_default_context(built_libs):
     [t.join() for t in ts]
     assert len({id(c) for c in (mine, *others)}) == 4
     assert default_context() is mine
+
+
+def test_a_release_reaches_the_default_contexts_of_other_threads(rt):
+    """Calls of a backward pass run on a thread of its own, and the step that releases runs on the main one. Their scratch is
+    free again at that thread's next call, not while a call of it is under way."""
+    from diopi_b200.runtime import default_context
+    calls, replies = queue.Queue(), queue.Queue()
+
+    def work():
+        while calls.get():
+            ctx = default_context()
+            replies.put((scratch(rt, ctx), ctx.stats()["blocks"]))
+
+    t = threading.Thread(target=work)
+    t.start()
+    try:
+        def call():
+            calls.put(True)
+            return replies.get(timeout=60)
+        first, _ = call()
+        assert call()[0] != first                 # not released
+        seen = set()
+        for _ in range(20):
+            default_context().release()
+            got, blocks = call()
+            seen.add(got)
+        assert len(seen) == 1 and blocks == 2
+    finally:
+        calls.put(False)
+        t.join()
 
 
 @pytest.mark.gpu
