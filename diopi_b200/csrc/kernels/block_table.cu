@@ -4,9 +4,10 @@
 // list in request order: first_i = free_start + sum of need_r over r < i.
 //
 // Bound by latency: launch, lengths, block ids, stores. A decode step of 64 requests takes 3.0 us, 64 prompts of up to 8192 tokens
-// 4.2, 1024 requests with the table of one slot for each token (16.8 MB) 14.5.
+// 4.2, 1024 requests with the table of one slot for each token (16.8 MB) 14.5 (64-bit indexes: 2.9, 4.2, 16.9).
 // One launch does everything: CTA (i, y) adds up need and n over the requests before i itself (B loads from L2, cheaper
-// than a second kernel or a wait between CTAs for any B that a batch has), then works on slice y of request i. Nothing
+// than a second kernel or a wait between CTAs for a thousand requests; the sums grow with B^2: a decode step of 2048
+// requests takes 10 us, of 8192 61, and 13 and 120 with 64-bit lengths), then works on slice y of request i. Nothing
 // it reads is written by another CTA: entries below have_i stay as they were, and the blocks behind them are read from
 // the free list, not from the table.
 #include "dev_util.cuh"

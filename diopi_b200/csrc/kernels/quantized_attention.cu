@@ -13,6 +13,10 @@
 // its factor; ref is only raised when a tile exceeds it by 2^16, or by less where values are above 2^41 (value_lift).
 // Queries are scaled by the power of two that brings their row's maximum to [1, 2) before they become fp16 (bf16 and fp32
 // reach further than fp16 does); fp32 queries and their weights are split into two fp16 numbers each, with two products.
+// What is rounded to fewer than 24 bits: a query element of bf16 or fp32 to 2^-25 of its row's largest where that is more than its
+// own last bits; a weight of fp16 or bf16 queries to one fp16 number (2^-11 of it). Against 64 bits the fp16 results of the third case
+// below are off by 2.7e-4 of their size on average, 2.1e-4 with weights in two parts, which is the rounding of the results
+// themselves (bf16: 1.7e-3 either way); two parts cost 19 % (70 to 83 us on the first case: spills at 128 registers).
 //
 // Work split: the tiles of the batch are cut into equal ranges, one per team, a team being the warps of one K/V head (one warp for up
 // to 8 * NT query rows, mt of them beyond). The teams of a CTA are hw neighbouring heads of the same range, which keeps their reads
@@ -22,16 +26,20 @@
 // ranges its parts are merged by quant_combine_kernel (a programmatic dependent launch); else it is written directly.
 //
 // Measured (calls one after the other in a graph, merge included): 64 query heads over 8 K/V heads, 64 requests of 512 to 4096
-// tokens, e4m3: 71 us = 4300 GB/s; a K/V head for each of 32 query heads, int8: 209 to 233 us on different GPUs = 0.79 to 0.88
-// of the copy rate; four requests of 30011 to 131072 tokens: 71 us. While it streams the loop runs at the copy rate (the loads alone take as long); what
-// is left is 5 us of start (lengths, block ids, first tiles), up to 9 us between the first SM's end and the last one's
+// tokens, bf16, e4m3: 70 us = 4350 GB/s; four requests of 30011 to 131072 tokens, fp16: 72 us; a K/V head for each of 32 query
+// heads, fp16, int8: 209 to 233 us on different GPUs = 0.79 to 0.88 of the copy rate. While it streams the loop runs at the copy
+// rate (the loads alone take as long); what is left is 5 us of start (lengths, block ids, first tiles), up to 9 us between the first SM's end and the last one's
 // (some groups of SMs get a tenth less bandwidth), 5 us of merge. Tried and dropped: query rows as the M extent (half of
 // the products on padding; 98 us); a producer warp beside 16 others (96 registers, spills: 124 us); the last eighth of each
 // range given away through clusterlaunchcontrol (79 us; 82 with the next piece's tiles fetched ahead); two CTAs of
 // eight warps an SM (the same time).
 //
-// quant_plain_kernel: any width, strides and block size; one CTA to a query row, a warp to every fourth token (the first case
-// above: 9854 us).
+// The new-token form for e4m3 at head_dim 128 spills 4 to 12 bytes a thread, fp32 queries 24 to 88 at head_dim 128 and 256, the
+// merge at 64 registers 68 to 72 (it asks for four parts at once; 32 warps an SM hide the rest).
+//
+// quant_plain_kernel: any width, strides and block size, and batches whose lengths the split kernel cannot hold (more than 4096);
+// one CTA to a query row, a warp to every fourth token (the first case above: 9854 us; 4097 requests of up to 60 tokens, 32
+// heads over 8: 4100 us, 4096 of them 170 on the split kernel).
 #include <cuda.h>
 
 #include <atomic>

@@ -11,9 +11,11 @@
 // Bytes: T * H * D * (e + 1) for each of K and V. One pass: the rows of a block stay in registers between the maximum and
 // the codes. A unit is one (request, block, head) of one matrix; 16 (8) rows of it belong to a warp, with 16 elements of a row to
 // a lane, and up to 8 warps share a unit through shared memory. Blocks of more rows than that are read twice (the second time from
-// L1/L2). Bound by memory latency over 24 warps an SM, then by its rate: 36864 tokens x 32 heads x 128, fp16 to int8: 171 us =
-// 5300 GB/s = 0.81 of the copy rate; 124971 tokens x 8 heads, fp16 to e4m3: 132 us, 0.89. On the way there: vectors side by side
-// in a lane instead of whole lines, 394 us; calls for the rare cases inside the loop (spills), 231.
+// L1/L2). Bound by memory latency over 24 warps an SM, then by its rate: 36864 tokens x 32 heads x 128, fp16 to int8: 165 us =
+// 5500 GB/s = 0.84 of the copy rate; 124971 tokens x 8 heads, fp16 to e4m3: 128 us, 0.91. With fewer than 8 heads some warps of a
+// CTA have none (4 heads 99 us, 2: 91, 1: 86). On the way there: vectors side by side in a lane instead of whole lines, 394 us;
+// calls for the rare cases inside the loop, 231; the element-wise rows inside the loop, 171. Up to 40 bytes a thread are still
+// spilled at 80 and 64 registers (head_dim to 128); more registers leave an SM fewer CTAs.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -271,7 +273,7 @@ __global__ void __launch_bounds__(kCopyThreads, copy_ctas<T>(LPR)) quantized_cop
     const bool full_width = a.D == 16 * LPR;
 
     // K and V one after the other, or (two CTAs along z) one of them. (The rows of both asked for before either is stored: 128
-    // registers, two CTAs an SM, 220 us on the prompts above.)
+    // registers, two CTAs an SM, 220 us on the prompts above when this form took 171.)
 #pragma unroll 1
     for (int m = blockIdx.z; m < 2; m += gridDim.z) {
         const int64_t pitch = a.src_s0[m];
@@ -438,7 +440,7 @@ void launch_rows(const QuantCopyArgs& a, int units, int sm_count, cudaStream_t s
         const int upc = kCopyWarps / w;
         const int y = (a.H + upc - 1) / upc;
         // Few CTAs: K and V side by side (64 requests of one token: 3.7 us, 4.8 one after the other); many: one look-up for both
-        // (the prompts above: 171 us, 198 side by side).
+        // (the prompts above: 198 us side by side when this form took 171).
         kern<<<dim3(units, y, static_cast<int64_t>(units) * y < 8 * sm_count ? 2 : 1), kCopyThreads, 0, st>>>(a);
     };
     constexpr int rows = warp_rows<T>(LPR);

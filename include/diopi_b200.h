@@ -262,8 +262,9 @@ diopiError_t diopiBuildBlockTable(diopiContextHandle_t ctx, diopiTensorHandle_t 
  * cached_lens[i] + t of request i; rows behind new_start[B] are not read. A block whose position 0 is written begins anew:
  * s = amax * (1 / 127), both roundings in fp32 (int8), the smallest power of two with amax <= 448 s (e4m3), 2^-126 at least, 0 when amax = 0,
  * with amax the largest finite magnitude of the call's rows in it. A block that holds earlier tokens keeps s, or grows it
- * by the smallest sufficient power of two and rounds the codes in front of the new rows to the grown scale. Codes are the
- * nearest to x / s, ties to even; infinities saturate, NaN becomes 0 (int8) or NaN (e4m3). Positions behind the new
+ * by the smallest sufficient power of two and rounds the codes in front of the new rows to the grown scale; s may be any
+ * finite number there, not only one of this op's. Codes are the nearest to x / s, ties to even, and 0 where s is 0;
+ * infinities saturate, NaN becomes 0 (int8) or NaN (e4m3). Positions behind the new
  * rows stay as they were. Two requests must not write one block in the same call; rows whose block is
  * outside the cache are skipped (status 1). */
 diopiError_t diopiQuantizedCopyKV(diopiContextHandle_t ctx, diopiTensorHandle_t k_cache, diopiTensorHandle_t v_cache, diopiTensorHandle_t k_scale,
@@ -273,8 +274,10 @@ diopiError_t diopiQuantizedCopyKV(diopiContextHandle_t ctx, diopiTensorHandle_t 
 /* diopiQuantizedPagedAttention: decode attention over such a cache. q, out [B, H, D] or [B, n, H, D] (fp16, bf16, fp32;
  * H a multiple of Hkv): the n newest tokens of each request, whose K/V rows are in the cache already. seq_lens [B] counts
  * all tokens of a request; token t of n sees the first seq_lens[i] - (n - 1 - t) of them, causally, and one that sees none
- * gets zeros. out = softmax(softmax_scale * q k^T) v with softmax_scale > 0. Scales must be finite and not negative. Tokens in a block
- * outside the cache are left out (status 1). */
+ * gets zeros; a length beyond the row of block_table counts as that row's. out = softmax(softmax_scale * q k^T) v with
+ * softmax_scale > 0. Scales must be finite and not negative, logits within 1e38 (with values above 1e23: within 1e8).
+ * Elements of bf16 and fp32 queries are held to 2^-25 of their row's largest magnitude. An infinity or a NaN in a row of q makes that
+ * row NaN. Tokens in a block outside the cache are left out (status 1). */
 diopiError_t diopiQuantizedPagedAttention(diopiContextHandle_t ctx, diopiTensorHandle_t out, diopiConstTensorHandle_t q, diopiConstTensorHandle_t k_cache,
                                           diopiConstTensorHandle_t v_cache, diopiConstTensorHandle_t k_scale, diopiConstTensorHandle_t v_scale,
                                           diopiConstTensorHandle_t block_table, diopiConstTensorHandle_t seq_lens, double softmax_scale);
