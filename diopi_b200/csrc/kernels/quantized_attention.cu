@@ -71,7 +71,8 @@ constexpr int kTile = 16;   // tokens of a tile
 constexpr float kLowest = -3e38f;   // below every logit, and finite
 
 // How far the reference of the weights has to be above a logit in a block of value scale s, so that a sum of weights times values
-// stays finite wherever their mean is: s * 2^-lift < 2^(from + 1). 0 for the values that a model has.
+// stays finite wherever their mean is: s * 2^-lift < 2^(from + 1). 0 for the values that a model has; else differences of logits are
+// taken at a distance of up to 86 from the reference, which rounds them to 2^-18.
 __device__ __forceinline__ float value_lift(float s, int from) { return static_cast<float>(max(static_cast<int>(__float_as_uint(s) << 1 >> 24) - 127 - from, 0)); }
 // What the reference of the split kernel may lag behind a tile's maximum. With a weight of 2^(15 + kLag - lift) at most the sum over
 // 2^31 tokens of code * s stays below 2^(31 + 9 + 42 + 31) = 2^113, and l above 2^(15 - 86).

@@ -12,7 +12,7 @@
 // the codes. A unit is one (request, block, head) of one matrix; 16 (8) rows of it belong to a warp, with 16 elements of a row to
 // a lane, and up to 8 warps share a unit through shared memory. Blocks of more rows than that are read twice (the second time from
 // L1/L2). Bound by memory latency over 24 warps an SM, then by its rate: 36864 tokens x 32 heads x 128, fp16 to int8: 165 us =
-// 5500 GB/s = 0.84 of the copy rate; 124971 tokens x 8 heads, fp16 to e4m3: 128 us, 0.91. With fewer than 8 heads some warps of a
+// 5500 GB/s = 0.84 of the copy rate; 124971 tokens x 8 heads, fp16 to e4m3: 128 us, 0.92. With fewer than 8 heads some warps of a
 // CTA have none (4 heads 99 us, 2: 91, 1: 86). On the way there: vectors side by side in a lane instead of whole lines, 394 us;
 // calls for the rare cases inside the loop, 231; the element-wise rows inside the loop, 171. Up to 40 bytes a thread are still
 // spilled at 80 and 64 registers (head_dim to 128); more registers leave an SM fewer CTAs.

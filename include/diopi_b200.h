@@ -275,7 +275,8 @@ diopiError_t diopiQuantizedCopyKV(diopiContextHandle_t ctx, diopiTensorHandle_t 
  * H a multiple of Hkv): the n newest tokens of each request, whose K/V rows are in the cache already. seq_lens [B] counts
  * all tokens of a request; token t of n sees the first seq_lens[i] - (n - 1 - t) of them, causally, and one that sees none
  * gets zeros; a length beyond the row of block_table counts as that row's. out = softmax(softmax_scale * q k^T) v with
- * softmax_scale > 0. Scales must be finite and not negative, logits within 1e38 (with values above 1e23: within 1e8).
+ * softmax_scale > 0. Scales must be finite and not negative, logits within 1e38 (with values above 1e23: within 1e8);
+ * where values are above 1e12, weights are held to 2^-18.
  * Elements of bf16 and fp32 queries are held to 2^-25 of their row's largest magnitude. An infinity or a NaN in a row of q makes that
  * row NaN. Tokens in a block outside the cache are left out (status 1). */
 diopiError_t diopiQuantizedPagedAttention(diopiContextHandle_t ctx, diopiTensorHandle_t out, diopiConstTensorHandle_t q, diopiConstTensorHandle_t k_cache,

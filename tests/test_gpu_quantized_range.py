@@ -68,7 +68,8 @@ def test_attention_of_huge_logits(F, ctx, n, e4m3, bs, D, dt, scale):  # noqa: F
 def test_attention_of_huge_values(F, ctx, n, e4m3, D, dt, factor):  # noqa: F811
     """Values that only the 8-bit exponent of bf16 and fp32 reaches, next to ordinary ones; logits that grow along the request,
     so that the running maximum rises a little with almost every tile. The bounds are those of any other value: all of
-    them are relative to sum p |v|, but the one of the weights' last bits, which goes by the value itself (sum |v|)."""
+    them are relative to sum p |v|, but the one of the weights' last bits, which goes by the value itself (sum |v|). (The 2^-18 to
+    which weights of such values are held are far below what logits of hundreds may be off by.)"""
     lens = [1, 17, 40, 333, 700, 0]
     q, kc, vc, ks, vs, table, lens_t = attention_inputs(lens, n=n, e4m3=e4m3, D=D, dt=dt, seed=D)
     for i, L in enumerate(lens):
@@ -81,6 +82,21 @@ def test_attention_of_huge_values(F, ctx, n, e4m3, D, dt, factor):  # noqa: F811
     mixed[::2] /= factor
     check_attention(F, ctx, (q, kc, vc, ks, mixed, table, lens_t))
     ctx.release()
+
+
+@pytest.mark.parametrize("factor", [1e13, 1e20, 1e34])
+@pytest.mark.parametrize("n,e4m3,D", [(1, True, 64), (3, True, 128), (1, False, 256), (2, False, 40)])
+def test_attention_of_huge_values_and_small_logits(F, ctx, n, e4m3, D, factor):  # noqa: F811
+    """fp32 queries so small that logits hardly matter: what is left is how exactly weights of such values are held. A weight is
+    2^(x - r) with x - r rounded at a magnitude below 128, by 2^-18, and its normaliser is a sum of such: 2 ln 2 * 2^-18 < 2^-17."""
+    lens = [1, 17, 40, 333, 700, 0]
+    q, kc, vc, ks, vs, table, lens_t = attention_inputs(lens, n=n, e4m3=e4m3, D=D, dt="fp32", seed=D, std=1e-4)
+    vs = vs.clamp(max=0.3) * factor / 3
+    vs[::2] /= factor
+    args = (q, kc, vc, ks, vs, table, lens_t)
+    want, sums = O.quantized_paged_attention(*args, 0.1)
+    got = F.quantized_paged_attention(*[t.cuda() for t in args], 0.1, ctx=ctx).cpu().double()
+    assert bool(((got - want).abs() <= bound_of(want, sums, 700, D, torch.float32) + sums[0] * 2.0 ** -17).all())
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
