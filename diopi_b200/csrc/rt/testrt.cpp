@@ -12,8 +12,9 @@
 // (b200rt_context_release) that the work using it was enqueued, and only for work on
 // the stream that used it before, where that work comes first (another stream's might
 // still be reading it). Two exceptions: a stream that is being captured cannot allocate
-// and takes any free block (a block that a graph uses is that stream's from then on),
-// and when memory is out a block of another stream is taken after the device is idle.
+// and takes any free block, and when memory is out a block of another stream is taken
+// after the device is idle. A block that a capture took serves captures only from then
+// on: its graph may be replayed on any stream, beside any call.
 #include <cuda_runtime_api.h>
 
 #include <algorithm>
@@ -45,6 +46,7 @@ struct Block {
     bool in_use = false;
     bool on_device = true;
     cudaStream_t stream = nullptr;   // whose work used it last
+    bool captured = false;           // a graph uses it
 };
 
 int64_t elem_size(diopiDtype_t dt) {
@@ -142,11 +144,11 @@ RT_EXPORT diopiError_t diopiGetStream(diopiContextHandle_t ctx, diopiStreamHandl
     return diopiSuccess;
 }
 
-// The smallest free block that holds `bytes`, of the context's stream or of any.
-static Block* free_block(diopiContextHandle_t ctx, int64_t bytes, bool on_device, bool any_stream) {
+// The smallest free block that holds `bytes`, of the context's stream or of any, in use by graphs or not.
+static Block* free_block(diopiContextHandle_t ctx, int64_t bytes, bool on_device, bool any_stream, bool captured) {
     Block* best = nullptr;
     for (auto& b : ctx->blocks) {
-        if (b.in_use || b.on_device != on_device || b.bytes < bytes || (!any_stream && b.stream != ctx->stream)) continue;
+        if (b.in_use || b.on_device != on_device || b.bytes < bytes || b.captured != captured || (!any_stream && b.stream != ctx->stream)) continue;
         if (!best || b.bytes < best->bytes) best = &b;
     }
     return best;
@@ -154,14 +156,24 @@ static Block* free_block(diopiContextHandle_t ctx, int64_t bytes, bool on_device
 
 static bool capturing(cudaStream_t stream) {
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-    return cudaStreamIsCapturing(stream, &status) == cudaSuccess && status == cudaStreamCaptureStatusActive;
+    if (cudaStreamIsCapturing(stream, &status) == cudaSuccess) return status == cudaStreamCaptureStatusActive;
+    cudaGetLastError();
+    return false;
 }
 
 static diopiError_t require_bytes(diopiContextHandle_t ctx, int64_t bytes, diopiDevice_t device, void** out) {
     ctx->n_require_calls++;
     const bool on_device = (device == diopi_device);
-    Block* best = free_block(ctx, bytes, on_device, false);
-    if (!best && on_device && capturing(ctx->stream)) best = free_block(ctx, bytes, on_device, true);
+    const bool capture = on_device && ctx->stream_ready && capturing(ctx->stream);
+    Block* best = nullptr;
+    if (capture) {   // the graphs of a context share, in the first place, what one of them has
+        best = free_block(ctx, bytes, on_device, false, true);
+        if (!best) best = free_block(ctx, bytes, on_device, false, false);
+        if (!best) best = free_block(ctx, bytes, on_device, true, false);
+        if (!best) best = free_block(ctx, bytes, on_device, true, true);
+    } else {
+        best = free_block(ctx, bytes, on_device, false, false);
+    }
     if (!best) {
         Block nb;
         nb.bytes = std::max<int64_t>(bytes, 256);
@@ -172,7 +184,7 @@ static diopiError_t require_bytes(diopiContextHandle_t ctx, int64_t bytes, diopi
             ctx->n_device_allocs++;
         } else {
             cudaGetLastError();
-            best = free_block(ctx, bytes, on_device, true);
+            best = free_block(ctx, bytes, on_device, true, false);
             if (!best || cudaDeviceSynchronize() != cudaSuccess) return diopiErrorOccurred;
         }
         if (!best) {
@@ -182,6 +194,7 @@ static diopiError_t require_bytes(diopiContextHandle_t ctx, int64_t bytes, diopi
     }
     best->in_use = true;
     best->stream = ctx->stream;
+    best->captured = best->captured || capture;
     *out = best->ptr;
     return diopiSuccess;
 }

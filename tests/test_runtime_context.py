@@ -155,3 +155,40 @@ def test_a_capture_takes_the_scratch_of_the_stream_that_warmed_up(built_libs):
         assert torch.equal(out, want) and torch.equal(other, want)
         out.zero_()
     assert ctx.stats()["device_allocs"] == allocs + 1
+
+
+@pytest.mark.gpu
+def test_calls_beside_a_graph_of_their_context(built_libs):
+    """The graph is replayed on another stream than the one it was captured on, where eager calls go on: they have scratch of their
+    own. Graphs captured one after the other share theirs."""
+    from diopi_b200 import functions as F
+    from diopi_b200.runtime import Context
+    from test_gpu_quantized_cache import attention_inputs
+    args = [[t.cuda() for t in attention_inputs([4000, 31, 700], seed=s)] for s in range(2)]
+    st, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        ctx = Context(st)
+        wants = [F.quantized_paged_attention(*a, 0.1, ctx=Context(st)) for a in args]
+        F.quantized_paged_attention(*args[0], 0.1, ctx=ctx)
+        outs = [torch.empty_like(w) for w in wants]
+        st.synchronize()
+        graphs = []
+        for _ in range(2):
+            ctx.release()
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=st):
+                F.quantized_paged_attention(*args[0], 0.1, ctx=ctx, out=outs[0])
+        ctx.release()
+        assert ctx.stats()["blocks"] == 1
+        eager = [torch.empty_like(wants[1]) for _ in range(40)]
+        F.quantized_paged_attention(*args[1], 0.1, ctx=ctx, out=eager[0])
+        assert ctx.stats()["blocks"] == 2
+        torch.cuda.synchronize()
+        for e in eager:
+            ctx.release()
+            F.quantized_paged_attention(*args[1], 0.1, ctx=ctx, out=e)
+            with torch.cuda.stream(other):
+                graphs[0].replay()
+        torch.cuda.synchronize()
+        assert ctx.stats()["blocks"] == 2
+        assert torch.equal(outs[0], wants[0]) and all(torch.equal(e, wants[1]) for e in eager)
