@@ -19,6 +19,8 @@ def _impl():
 def _t(x, as_device=None):
     if x is None or isinstance(x, Tensor):
         return x
+    if x.dtype == torch.float8_e4m3fn:   # only the ops on 8-bit caches, which do not come here, take its bits for uint8
+        raise TypeError(f"dtype {x.dtype} has no DIOPI counterpart")
     return Tensor(x, as_device=as_device)
 
 

@@ -40,7 +40,8 @@ _TORCH_TO_DIOPI = {
     torch.int64: Dtype.int64, torch.float16: Dtype.float16, torch.float32: Dtype.float32,
     torch.float64: Dtype.float64, torch.bool: Dtype.bool, torch.bfloat16: Dtype.bfloat16,
 }
-# The interface has no 8-bit float: the ops on 8-bit caches take the bits of e4m3 codes as uint8. Only theirs.
+# The interface has no 8-bit float: the ops on 8-bit caches take the bits of e4m3 codes as uint8. Only theirs, and handles that are
+# made by hand.
 _CODES_TO_DIOPI = {**_TORCH_TO_DIOPI, torch.float8_e4m3fn: Dtype.uint8}
 
 SUCCESS, ERROR_OCCURRED, NO_IMPLEMENT, DTYPE_NOT_SUPPORTED = 0, 1, 13, 1000
@@ -59,7 +60,7 @@ class Tensor:
 
     def __init__(self, t: torch.Tensor, *, as_device: bool | None = None):
         libs = _lib.load()
-        if t.dtype not in _TORCH_TO_DIOPI:
+        if t.dtype not in _CODES_TO_DIOPI:
             raise TypeError(f"dtype {t.dtype} has no DIOPI counterpart")
         self.torch = t  # keeps the memory alive
         nd = t.dim()
@@ -68,7 +69,7 @@ class Tensor:
         device = 1 if (t.is_cuda if as_device is None else as_device) else 0
         self._rt = libs.rt
         self.handle = libs.rt.b200rt_tensor_create(
-            ctypes.c_void_p(t.data_ptr()), nd, shape, stride, _TORCH_TO_DIOPI[t.dtype], device
+            ctypes.c_void_p(t.data_ptr()), nd, shape, stride, _CODES_TO_DIOPI[t.dtype], device
         )
 
     def __del__(self):
@@ -150,10 +151,11 @@ class _DefaultContext(Context):
         self.device, self.release_due = device, False
 
     def release(self) -> None:
-        super().release()
-        for other in list(_default_ctx.values()):
-            if other is not self and other.device == self.device:
-                other.release_due = True
+        self._rt.b200rt_context_release(self.handle)
+        if len(_default_ctx) > 1:
+            for other in list(_default_ctx.values()):
+                if other is not self and other.device == self.device:
+                    other.release_due = True
 
 
 _default_ctx: dict[tuple[int, int], _DefaultContext] = {}
